@@ -1,0 +1,39 @@
+// Element types of the fine-tuning kernels: bf16, fp16 and fp32 values that
+// are read and written 16 bytes at a time and computed on in fp32.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+namespace elem {
+
+template <typename T, int N>
+using vec = T __attribute__((ext_vector_type(N)));
+
+// elements of one 16-byte access
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+inline hipStream_t stream() {
+  return at::hip::getCurrentHIPStream().stream();
+}
+
+inline bool aligned16(const void* p) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+}  // namespace elem
+
+// Runs `...` with T bound to the device type of a torch scalar type.
+#define STOKE_ELEM_SWITCH(DTYPE, WHAT, ...)                              \
+  switch (DTYPE) {                                                       \
+    case at::kBFloat16: { using T = __bf16; __VA_ARGS__; break; }        \
+    case at::kHalf: { using T = _Float16; __VA_ARGS__; break; }          \
+    case at::kFloat: { using T = float; __VA_ARGS__; break; }            \
+    default:                                                             \
+      TORCH_CHECK(false, WHAT ": bf16, fp16 or fp32 tensors, got ",      \
+                  DTYPE);                                                \
+  }

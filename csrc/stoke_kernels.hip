@@ -690,6 +690,12 @@ at::Tensor fp8_quant(at::Tensor x, at::Tensor scale, at::Tensor amax_next,
 std::vector<at::Tensor> fp8_quant_t(at::Tensor x, at::Tensor scale,
                                     at::Tensor amax_next, int64_t kind);
 
+// Activations held in 8 bits (csrc/act8.hip)
+std::vector<at::Tensor> act8_pack(at::Tensor x);
+at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype);
+std::vector<at::Tensor> swiglu8_fwd(at::Tensor g, at::Tensor u);
+std::vector<at::Tensor> swiglu8_bwd(at::Tensor dy, at::Tensor held);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &ce_fwd, "fused bf16 cross-entropy forward (online lse)");
   m.def("ce_bwd", &ce_bwd, "fused bf16 cross-entropy backward");
@@ -737,5 +743,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused AdamW, bf16 params + fp32 master (HIP)");
   m.def("amp_update_scale_", &amp_update_scale_,
         "dynamic loss scale update (HIP)");
+  m.def("act8_pack", &act8_pack, "activation to 8 bits (MXINT8)");
+  m.def("act8_unpack", &act8_unpack, "activation back from 8 bits (MXINT8)");
+  m.def("swiglu8_fwd", &swiglu8_fwd,
+        "silu(g)*u, keeping g and u in 8 bits for the backward");
+  m.def("swiglu8_bwd", &swiglu8_bwd, "SwiGLU backward from 8-bit inputs");
   m.attr("_built_for") = "gfx950";
 }

@@ -39,7 +39,9 @@ setup(
                      "csrc/fa_fwd.hip",
                      "csrc/fa_bwd.hip",
                      "csrc/fp8_quant.hip",
-                     "csrc/fused_ce.hip"],
+                     "csrc/fused_ce.hip",
+                     "csrc/act8.hip"],
+            depends=["csrc/elem.h"],
             extra_compile_args={
                 "cxx": ["-O3"],
                 # scalar fp32 only: some packed fp32 forms the compiler makes

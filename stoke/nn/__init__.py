@@ -1,4 +1,9 @@
 from stoke.nn.act_ckpt import apply_activation_checkpointing  # noqa: F401
+from stoke.nn.act8 import (  # noqa: F401
+    CompressedActivation,
+    compress_activation,
+    restore_activation,
+)
 from stoke.nn.fused_bn import FusedBNAct2d  # noqa: F401
 from stoke.nn.layernorm import StokeLayerNorm  # noqa: F401
 from stoke.nn.rmsnorm import StokeRMSNorm  # noqa: F401

@@ -11,6 +11,10 @@ wrapped block for not storing its activations — on MI355X the recompute is
 usually HBM-resident and cheap relative to the 288 GB it frees for larger
 batches/models.
 
+``save_bits=8`` keeps the wrapped block's input activations in 8 bits
+(``stoke.nn.act8``): half the bytes of a 16-bit checkpoint.  The forward runs
+on the exact inputs; the recompute starts from the values held.
+
 Composes with the FSDP engine: the recompute re-fires the unit's
 forward-pre hook, which re-gathers the flat-param shard it needs.
 """
@@ -22,11 +26,71 @@ import torch
 import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
+from stoke.nn.act8 import (
+    check_save_bits,
+    compress_activation,
+    restore_activation,
+)
 
 _MARK = "_stoke_act_ckpt"
+_BITS = "_stoke_act_ckpt_bits"
 
 
-def _wrap_module(m: nn.Module) -> None:
+class _StandIn(torch.autograd.Function):
+    """A tensor of x's shape without its memory, through which the gradient
+    for x flows; the checkpoint keeps it in x's place."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.new_zeros(()).expand(x.shape)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad
+
+
+class _FillIn(torch.autograd.Function):
+    """The block's input in place of its stand-in: the exact one in the
+    forward pass, the one held in 8 bits in a recompute."""
+
+    @staticmethod
+    def forward(ctx, stand_in, held, exact):
+        if exact:
+            return exact.pop().detach()
+        return restore_activation(held)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad, None, None
+
+
+def _holds(t) -> bool:
+    # computed activations only: parameters, caller-held leaves, masks and
+    # tables stay alive elsewhere, so compressing them would add memory
+    return (isinstance(t, torch.Tensor) and t.grad_fn is not None
+            and t.dtype in (torch.bfloat16, torch.float16, torch.float32))
+
+
+def _checkpoint8(fn, args, kwargs):
+    """``checkpoint(fn, *args, **kwargs)`` with the activations among the
+    arguments held in 8 bits until the backward pass."""
+    flat = list(args) + list(kwargs.values())
+    held = {i: (compress_activation(t), [t]) for i, t in enumerate(flat)
+            if _holds(t)}
+    kept = [_StandIn.apply(t) if i in held else t for i, t in enumerate(flat)]
+    n, names = len(args), list(kwargs)
+    del flat, args, kwargs
+
+    def run(*vals):
+        vals = [_FillIn.apply(t, *held[i]) if i in held else t
+                for i, t in enumerate(vals)]
+        return fn(*vals[:n], **dict(zip(names, vals[n:])))
+
+    return checkpoint(run, *kept, use_reentrant=False)
+
+
+def _wrap_module(m: nn.Module, save_bits: int = 16) -> None:
+    setattr(m, _BITS, save_bits)  # of the last call, also when wrapped
     if getattr(m, _MARK, False):
         return
     inner_forward = m.forward
@@ -35,6 +99,8 @@ def _wrap_module(m: nn.Module) -> None:
     def ckpt_forward(*args, **kwargs):
         if not torch.is_grad_enabled() or not m.training:
             return inner_forward(*args, **kwargs)
+        if getattr(m, _BITS) == 8:
+            return _checkpoint8(inner_forward, args, kwargs)
         return checkpoint(
             inner_forward, *args, use_reentrant=False, **kwargs
         )
@@ -47,14 +113,18 @@ def apply_activation_checkpointing(
     model: nn.Module,
     predicate: Optional[Callable[[str, nn.Module], bool]] = None,
     min_params: int = 1_000_000,
+    save_bits: int = 16,
 ) -> int:
     """Wrap eligible submodules with recompute-in-backward.
 
     Default eligibility: any non-container child subtree holding at least
     ``min_params`` parameters (the same granularity the FSDP engine uses for
     shard units).  A custom ``predicate(name, module)`` overrides it.
+    ``save_bits=8`` holds the blocks' input activations in 8 bits (see the
+    module docstring); 16 keeps them as they are.
     Returns the number of modules wrapped.
     """
+    check_save_bits(save_bits)
     wrapped = 0
     visited = set()
 
@@ -62,7 +132,7 @@ def apply_activation_checkpointing(
         nonlocal wrapped
         if predicate is not None:
             if predicate(name, m):
-                _wrap_module(m)
+                _wrap_module(m, save_bits)
                 wrapped += 1
                 return True
             return False
@@ -70,7 +140,7 @@ def apply_activation_checkpointing(
             return False
         n = sum(p.numel() for p in m.parameters())
         if n >= min_params:
-            _wrap_module(m)
+            _wrap_module(m, save_bits)
             wrapped += 1
             return True
         return False

@@ -1,0 +1,393 @@
+# -*- coding: utf-8 -*-
+"""Activations held in 8 bits: the format, SwiGLU and the checkpoints that
+use it (CPU steps here, HIP kernels in the gpu tier) against float64."""
+
+import math
+
+import pytest
+import torch
+
+from stoke.nn import (
+    CompressedActivation,
+    apply_activation_checkpointing,
+    compress_activation,
+    restore_activation,
+    swiglu,
+)
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+# around a block of 32, around 16-byte pieces, several blocks of threads
+SIZES = [(1,), (31,), (32,), (33,), (5, 7), (3, 64), (2, 3, 100), (4, 4096),
+         (257, 1367)]
+
+
+def _skip(device):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def _act(shape, dtype, device, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g)
+    x = x * torch.exp(2 * torch.randn(shape[-1], generator=g))
+    return x.to(dtype).to(device)
+
+
+def _blocks64(x):
+    v = x.detach().cpu().double().flatten()
+    return torch.nn.functional.pad(v, (0, -v.numel() % 32)).view(-1, 32)
+
+
+def _held64(x):
+    """(values, exponents) by the definition, in Python numbers."""
+    blk = _blocks64(x)
+    out, exps = torch.empty_like(blk), []
+    for i, row in enumerate(blk.tolist()):
+        top = max(abs(v) for v in row)
+        e = max(math.frexp(top)[1] - 7, -126) if top else -126
+        if round(math.ldexp(top, -e)) > 127:
+            e += 1
+        exps.append(e + 127)
+        out[i] = torch.tensor(
+            [math.ldexp(round(math.ldexp(v, -e)), e) for v in row],
+            dtype=torch.float64)
+    return out.view(-1)[: x.numel()].view(x.shape), exps
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SIZES)
+def test_format_matches_definition(shape, dtype, device):
+    _skip(device)
+    x = _act(shape, dtype, device)
+    held = compress_activation(x)
+    want, exps = _held64(x)
+    assert held.values.dtype == torch.int8 and held.values.shape == x.shape
+    assert held.scales.tolist() == exps
+    assert int(held.values.abs().max()) <= 127
+    back = restore_activation(held)
+    assert back.dtype == dtype and back.shape == x.shape
+    # 7 bits fit into every dtype above its subnormals: equal, one rounding
+    assert torch.equal(back.cpu().double(), want.to(dtype).double())
+    # the bound the format promises: half a step, 1/127 of the block's top
+    off = (_blocks64(back) - _blocks64(x)).abs()
+    assert bool((off <= _blocks64(x).abs().amax(-1, keepdim=True) / 127).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_format_at_the_ends_of_the_range(dtype, device):
+    _skip(device)
+    fin = torch.finfo(dtype)
+    x = torch.zeros(7, 32, dtype=dtype)
+    x[0, 3] = fin.max
+    x[1, 5], x[1, 6] = -fin.max, fin.max / 2
+    x[2] = fin.tiny
+    x[3, 0] = fin.tiny * 2.0 ** -(7 if dtype != torch.float16 else 10)
+    x[4] = -0.0
+    x[5] = torch.linspace(-1, 1, 32)
+    x[6, :2] = torch.tensor([127.5, 1.5]).to(dtype)  # 127.5 rounds past 127
+    x = x.to(device)
+    held = compress_activation(x)
+    want, exps = _held64(x)
+    assert held.scales.tolist() == exps
+    back = restore_activation(held)
+    assert torch.isfinite(back).all()
+    # the largest value rounds to a power of two out of range: it comes back
+    want = want.clamp(-fin.max, fin.max)
+    assert torch.equal(back.cpu().double(), want.to(dtype).double())
+    assert float(back[0, 3]) == fin.max and float(back[1, 5]) == -fin.max
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_non_finite_blocks_read_back_as_nan(bad, dtype, device):
+    _skip(device)
+    x = torch.ones(100, dtype=dtype)
+    x[40] = bad
+    back = restore_activation(compress_activation(x.to(device))).cpu()
+    assert torch.isnan(back[32:64]).all()
+    assert torch.equal(back[:32], x[:32]) and torch.equal(back[64:], x[64:])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty_and_strided_and_offset_inputs(device):
+    _skip(device)
+    e = compress_activation(torch.empty(0, 5, device=device))
+    assert restore_activation(e).shape == (0, 5)
+    base = _act((40, 66), torch.bfloat16, device)
+    for x in (base.t(), base[:, 1:], base[1:, ::2], base.flatten()[3:]):
+        a, b = compress_activation(x), compress_activation(x.clone(
+            memory_format=torch.contiguous_format))
+        assert torch.equal(a.values, b.values)
+        assert torch.equal(a.scales, b.scales)
+
+
+def test_refusals():
+    with pytest.raises(ValueError):
+        compress_activation(torch.zeros(4, dtype=torch.float64))
+    held = compress_activation(torch.zeros(40))
+    with pytest.raises(ValueError):
+        restore_activation(CompressedActivation(
+            held.values, held.scales[:1], held.dtype))
+    with pytest.raises(ValueError):
+        restore_activation(CompressedActivation(
+            held.values.float(), held.scales, held.dtype))
+    with pytest.raises(ValueError):
+        restore_activation(CompressedActivation(
+            held.values, held.scales, torch.int32))
+    with pytest.raises(ValueError):
+        swiglu(torch.zeros(4), torch.zeros(4), save_bits=4)
+    with pytest.raises(ValueError):
+        swiglu(torch.zeros(4, 4), torch.zeros(4), save_bits=8)
+    with pytest.raises(ValueError):
+        swiglu(torch.zeros(4), torch.zeros(4).half(), save_bits=8)
+    with pytest.raises(ValueError):
+        apply_activation_checkpointing(torch.nn.Linear(2, 2), save_bits=12)
+
+
+# ------------------------------------------------------------------ SwiGLU
+def _steps(g):
+    # fp32 steps, in units of 2^-24: e^-g from exp2 is off by |g| (rounding
+    # of g log2 e) + 0.25 |g| (log2 e itself) + 2; a sum, a quotient (2 ulp)
+    # and up to 4 products follow.  1 - s loses up to |g| more in g (1 - s).
+    return (24 + 4 * g.detach().abs()) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SIZES)
+def test_swiglu8_against_float64(shape, dtype, device):
+    _skip(device)
+    g = _act(shape, dtype, device, 1).clamp(-40, 40).requires_grad_(True)
+    u = _act(shape, dtype, device, 2).clamp(-40, 40).requires_grad_(True)
+    dy = _act(shape, dtype, device, 3).clamp(-4, 4)
+    y = swiglu(g, u, save_bits=8)
+    y.backward(dy)
+
+    def f(a, b):
+        return a * torch.sigmoid(a) * b
+
+    tiny = torch.finfo(dtype).tiny
+    tol = torch.finfo(dtype).eps / 2 + _steps(g.cpu().double())
+    want = f(g.detach().cpu().double(), u.detach().cpu().double())
+    off = (y.detach().cpu().double() - want).abs()
+    # below the smallest normal number a rounding is absolute
+    assert bool((off <= tol * want.abs() + tiny * tol).all())
+    hg = _held64(g)[0].requires_grad_(True)
+    hu = _held64(u)[0].requires_grad_(True)
+    dg, du = torch.autograd.grad(f(hg, hu), (hg, hu), dy.cpu().double())
+    # 1 + g (1 - s) cancels near its root at g = -1.28: its error is relative
+    # to the terms, |dy u s| (1 + |g| (1 - s))
+    s = torch.sigmoid(hg)
+    size = (dy.cpu().double() * hu * s).abs() * (1 + hg.abs() * (1 - s))
+    slack = _steps(hg) * size.detach()
+    off = (g.grad.cpu().double() - dg).abs()
+    assert bool((off <= tol * dg.abs() + slack + tiny * tol).all())
+    off = (u.grad.cpu().double() - du).abs()
+    assert bool((off <= tol * du.abs() + tiny * tol).all())
+
+
+def test_swiglu8_gradient_against_differences():
+    # whole multiples of 1/64 below 2 are held exactly
+    g = torch.randint(-100, 101, (3, 40)).double() / 64
+    u = torch.randint(-100, 101, (3, 40)).double() / 64
+    g[:, 0] = u[:, 0] = g[:, 32] = u[:, 32] = 1.75
+    gf, uf = g.float().requires_grad_(True), u.float().requires_grad_(True)
+    swiglu(gf, uf, save_bits=8).sum().backward()
+    h = 1e-5
+
+    def f(a, b):
+        return a * torch.sigmoid(a) * b
+
+    dg = (f(g + h, u) - f(g - h, u)) / (2 * h)
+    du = (f(g, u + h) - f(g, u - h)) / (2 * h)
+    # differences: h^2 f'''/6 < 1e-10 and 2^-53 |f| / h < 1e-10; fp32: 24 ulp
+    # of terms up to 2 * 1.75
+    assert (gf.grad.double() - dg).abs().max() < 24 * 2.0 ** -24 * 4
+    assert (uf.grad.double() - du).abs().max() < 24 * 2.0 ** -24 * 4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_swiglu8_strided_gradient_and_halves_of_one_projection(device):
+    _skip(device)
+    both = _act((6, 2 * 96), torch.bfloat16, device).requires_grad_(True)
+    g, u = both.chunk(2, -1)
+    y = swiglu(g, u, save_bits=8)
+    dy = _act((96, 6), torch.bfloat16, device, 5).t()
+    grad, = torch.autograd.grad(y, both, dy)
+    gc = g.detach().contiguous().requires_grad_(True)
+    uc = u.detach().contiguous().requires_grad_(True)
+    yc = swiglu(gc, uc, save_bits=8)
+    dg, du = torch.autograd.grad(yc, (gc, uc), dy.contiguous())
+    assert torch.equal(y, yc)
+    assert torch.equal(grad, torch.cat((dg, du), -1))
+
+
+# -------------------------------------------------------------- checkpoints
+class _Block(torch.nn.Module):
+    def __init__(self, d):
+        super().__init__()
+        self.a = torch.nn.Linear(d, d)
+        self.b = torch.nn.Linear(d, d)
+        self.drop = torch.nn.Dropout(0.2)
+        self.calls = []
+
+    def forward(self, x, shift, scale=None, flag=True):
+        self.calls.append(x.detach().clone())
+        assert flag
+        y = self.drop(torch.tanh(self.a(x))) + shift
+        return x + self.b(y) * scale
+
+
+class _Net(torch.nn.Module):
+    def __init__(self, d=40, n=3):
+        super().__init__()
+        self.blocks = torch.nn.ModuleList([_Block(d) for _ in range(n)])
+
+    def forward(self, x, shift, scale):
+        for blk in self.blocks:
+            x = blk(x, shift, scale=scale, flag=True)
+        return x
+
+
+def _run_net(device, bits, x, shift, scale):
+    torch.manual_seed(3)
+    net = _Net().to(device)
+    if bits:
+        apply_activation_checkpointing(
+            net, predicate=lambda n, m: isinstance(m, _Block),
+            save_bits=bits)
+    out = net(x * 1.0, shift, scale)
+    return net, out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_checkpoint8_runs_exact_forward_and_held_recompute(device):
+    _skip(device)
+    x = _act((5, 7, 40), torch.float32, device).clamp(-2, 2)
+    shift = torch.randn(40, generator=torch.Generator().manual_seed(9)).to(
+        device)
+    x.requires_grad_(True)
+    scale = torch.full((), 0.5, device=device, requires_grad=True)
+    plain, out = _run_net(device, 0, x, shift, scale)
+    want = torch.autograd.grad(out.square().sum(),
+                               [x, scale, *plain.parameters()])
+    net, got_out = _run_net(device, 8, x, shift, scale)
+    assert torch.equal(out, got_out)  # the forward sees the exact inputs
+    got = torch.autograd.grad(got_out.square().sum(),
+                              [x, scale, *net.parameters()])
+    for i, blk in enumerate(net.blocks):
+        first, again = blk.calls
+        assert torch.equal(
+            again, restore_activation(compress_activation(first)))
+        assert torch.equal(first, plain.blocks[i].calls[0])
+    for a, b in zip(got, want):
+        assert a.shape == b.shape
+        assert not torch.isnan(a).any()
+        # inputs are off by 1/127 of a block's largest: the gradients follow
+        # them, they are not those of another function
+        assert float((a - b).norm() / b.norm()) < 0.05
+
+
+def test_checkpoint8_gradients_are_those_at_the_held_values():
+    # inputs that 8 bits hold exactly: bit-equal gradients
+    x = (torch.randint(-127, 128, (4, 40)) / 64).float()
+    x[:, ::8] = 1.75
+    w = torch.randn(40, 40)
+
+    class Lin(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.Parameter(w.clone())
+
+        def forward(self, x):
+            return torch.tanh(x @ self.w)
+
+    nets = [torch.nn.Sequential(Lin()) for _ in range(2)]
+    apply_activation_checkpointing(nets[1], predicate=lambda n, m: True,
+                                   save_bits=8)
+    grads = []
+    for net in nets:
+        leaf = x.clone().requires_grad_(True)
+        net(leaf * 1.0).sum().backward()
+        grads.append((leaf.grad, net[0].w.grad))
+    assert torch.equal(grads[0][0], grads[1][0])
+    assert torch.equal(grads[0][1], grads[1][1])
+
+
+def test_checkpoint8_keeps_no_other_copy_of_its_input():
+    import gc
+    import weakref
+
+    seen = []
+
+    class Ident(torch.nn.Module):
+        def forward(self, x):
+            return x.square()
+
+    net = torch.nn.Sequential(Ident())
+    apply_activation_checkpointing(net, predicate=lambda n, m: True,
+                                   save_bits=8)
+    leaf = torch.randn(64, requires_grad=True)
+    x = leaf * 2.0
+    seen.append(weakref.ref(x))
+    y = net(x)
+    del x
+    gc.collect()
+    assert seen[0]() is None
+    y.sum().backward()
+    assert leaf.grad is not None
+
+
+def test_checkpoint8_eval_no_grad_and_change_of_bits():
+    net = _Net().train()
+    n = apply_activation_checkpointing(
+        net, predicate=lambda n, m: isinstance(m, _Block), save_bits=8)
+    assert n == 3
+    apply_activation_checkpointing(
+        net, predicate=lambda n, m: isinstance(m, _Block))
+    x = torch.randn(2, 40, requires_grad=True)
+    net(x * 1.0, torch.zeros(40), torch.ones(())).sum().backward()
+    # back at 16 bits: the recompute sees the exact input
+    first, again = net.blocks[0].calls
+    assert torch.equal(first, again)
+    net.eval()
+    with torch.no_grad():
+        net(x, torch.zeros(40), torch.ones(()))
+    assert len(net.blocks[0].calls) == 3
+
+
+@pytest.mark.gpu
+def test_gpu_checkpoint8_saves_memory_under_autocast():
+    _skip("cuda")
+    d, n = 1024, 6
+
+    class Mlp(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = torch.nn.Linear(d, d)
+
+        def forward(self, x):
+            return x + torch.tanh(self.a(x))
+
+    held = {}
+    for bits in (16, 8):
+        torch.manual_seed(0)
+        net = torch.nn.Sequential(*[Mlp() for _ in range(n)]).cuda().bfloat16()
+        apply_activation_checkpointing(
+            net, predicate=lambda n, m: isinstance(m, Mlp), save_bits=bits)
+        leaf = torch.randn(8192, d, device="cuda", dtype=torch.bfloat16,
+                           requires_grad=True)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = net(leaf * 1.0)
+        held[bits] = torch.cuda.memory_allocated() - before
+        y.float().square().mean().backward()
+        assert torch.isfinite(leaf.grad).all()
+    # n inputs of 2 bytes against 1 1/32, and the output of both
+    per = 8192 * d
+    assert held[16] >= (n + 1) * 2 * per
+    assert held[8] <= n * per * 33 / 32 + 2 * per + (1 << 22)
