@@ -696,6 +696,22 @@ at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype);
 std::vector<at::Tensor> swiglu8_fwd(at::Tensor g, at::Tensor u);
 std::vector<at::Tensor> swiglu8_bwd(at::Tensor dy, at::Tensor held);
 
+// Token log-probabilities and the losses on them (csrc/token_loss.hip)
+std::vector<at::Tensor> token_logprobs_fwd(at::Tensor logits,
+                                           at::Tensor target,
+                                           int64_t ignore);
+std::vector<at::Tensor> policy_loss_fwd(
+    at::Tensor logits, at::Tensor target, at::Tensor old_lp, at::Tensor adv,
+    c10::optional<at::Tensor> ref_lp, double low, double high, double kl,
+    int64_t ignore);
+std::vector<at::Tensor> preference_loss_fwd(at::Tensor logits,
+                                            at::Tensor target,
+                                            at::Tensor ref_lp, double beta,
+                                            double eps, int64_t ignore);
+at::Tensor token_loss_bwd(at::Tensor logits, at::Tensor target,
+                          at::Tensor saved, at::Tensor up,
+                          c10::optional<at::Tensor> scale, int64_t ignore);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &ce_fwd, "fused bf16 cross-entropy forward (online lse)");
   m.def("ce_bwd", &ce_bwd, "fused bf16 cross-entropy backward");
@@ -748,5 +764,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu8_fwd", &swiglu8_fwd,
         "silu(g)*u, keeping g and u in 8 bits for the backward");
   m.def("swiglu8_bwd", &swiglu8_bwd, "SwiGLU backward from 8-bit inputs");
+  m.def("token_logprobs_fwd", &token_logprobs_fwd,
+        "log-probabilities of given tokens");
+  m.def("policy_loss_fwd", &policy_loss_fwd,
+        "clipped policy loss with a KL term, forward");
+  m.def("preference_loss_fwd", &preference_loss_fwd,
+        "paired preference loss, forward");
+  m.def("token_loss_bwd", &token_loss_bwd,
+        "logits' gradient of a loss on token log-probabilities");
   m.attr("_built_for") = "gfx950";
 }

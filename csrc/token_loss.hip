@@ -1,0 +1,499 @@
+// Log-probabilities of given tokens, and the losses built on them (MI355X).
+//
+// For a row of logits x and a token t, with M = max x:
+//   lp = x_t - M - log sum_j exp(x_j - M)
+//   d lp / d x_j = [j = t] - exp(x_j - M) / sum
+// Every loss here is a function of the lp alone, so a step is three passes
+// over memory: the forward reads the logits once (running maximum and sum),
+// a finishing kernel turns the row statistics into lp, the loss and each
+// row's d loss / d lp, and the backward reads the logits once more and
+// writes the gradient.  Rows whose target is ignored are not read, nor, in
+// the backward, rows whose coefficient is zero (clipped tokens): their
+// gradient is written as zeros.
+//
+// The sum of exponentials is kept in fp32; what follows it (log, differences
+// to other log-probabilities, sums over tokens) is done in fp64, because the
+// losses take small differences of large sums.
+
+#include <hip/hip_runtime.h>
+
+#include "elem.h"
+
+namespace {
+
+using elem::kVec;
+
+constexpr int kThreads = 256;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+struct Shape {
+  long rows, vocab;        // rows = outer * inner
+  long inner;              // rows that follow each other at row_stride
+  long outer_stride, row_stride;  // of the logits, in elements
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const T* x, const Shape& s,
+                                           long row) {
+  return x + (row / s.inner) * s.outer_stride +
+         (row % s.inner) * s.row_stride;
+}
+
+__device__ __forceinline__ bool is_live(long t, long vocab, long ignore) {
+  return t != ignore && t >= 0 && t < vocab;
+}
+
+// (M, sum) of two pieces of a row.  A piece without a finite maximum keeps
+// its sum as it is: exp(-inf - -inf) would be NaN where nothing was seen.
+__device__ __forceinline__ void join(float& m, float& s, float mo, float so) {
+  const float top = fmaxf(m, mo);
+  const float a = m == top ? 1.f : __expf(m - top);
+  const float b = mo == top ? 1.f : __expf(mo - top);
+  s = s * a + so * b;
+  m = top;
+}
+
+// One block for each (row, piece of the vocabulary): stats[row, piece].
+template <typename T>
+__global__ __launch_bounds__(kThreads) void row_stats_kernel(
+    const T* __restrict__ logits, const long* __restrict__ target,
+    float2* __restrict__ stats, unsigned* __restrict__ ticket, Shape s,
+    long ignore, int pieces, long piece) {
+  const long row = blockIdx.x;
+  const int part = blockIdx.y;
+  if (row == 0 && part == 0 && threadIdx.x == 0 && ticket) *ticket = 0;
+  if (!is_live(target[row], s.vocab, ignore)) return;
+  const T* x = row_of(logits, s, row);
+  const long end = min(s.vocab, (part + 1) * piece);
+  float m = kNegInf, sum = 0.f;
+  for (long i = part * piece + threadIdx.x; i < end; i += kThreads) {
+    const float v = (float)x[i];
+    if (v > m) {
+      sum *= __expf(m - v);
+      m = v;
+    }
+    // +inf - +inf: the row has no distribution, NaN as torch has it
+    if (v != kNegInf) sum += __expf(v - m);
+  }
+  #pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    join(m, sum, __shfl_xor(m, off), __shfl_xor(sum, off));
+  __shared__ float2 part_stats[kThreads / 64];
+  if ((threadIdx.x & 63) == 0)
+    part_stats[threadIdx.x >> 6] = make_float2(m, sum);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    #pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w)
+      join(m, sum, part_stats[w].x, part_stats[w].y);
+    stats[row * pieces + part] = make_float2(m, sum);
+  }
+}
+
+struct RowLp {
+  float m, inv;  // maximum, 1 / sum
+  double lp;
+};
+
+// Joins the pieces of a row in their order.
+template <typename T>
+__device__ __forceinline__ RowLp row_lp(const T* __restrict__ logits,
+                                        const float2* __restrict__ stats,
+                                        const Shape& s, long row, long t,
+                                        int pieces) {
+  float2 a = stats[row * pieces];
+  for (int p = 1; p < pieces; ++p) {
+    const float2 b = stats[row * pieces + p];
+    join(a.x, a.y, b.x, b.y);
+  }
+  RowLp r;
+  r.m = a.x;
+  r.inv = 1.f / a.y;
+  r.lp = (double)((float)row_of(logits, s, row)[t]) - (double)a.x -
+         log((double)a.y);
+  return r;
+}
+
+// What the backward needs of a row: maximum, 1 / sum, lp and (for the
+// losses) the row's coefficient.
+struct Saved {
+  float m, inv, lp, coef;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void lp_finish_kernel(
+    const T* __restrict__ logits, const long* __restrict__ target,
+    const float2* __restrict__ stats, float4* __restrict__ saved,
+    float* __restrict__ lp, Shape s, long ignore, int pieces) {
+  const long row = (long)blockIdx.x * kThreads + threadIdx.x;
+  if (row >= s.rows) return;
+  const long t = target[row];
+  if (!is_live(t, s.vocab, ignore)) {
+    lp[row] = 0.f;
+    saved[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    return;
+  }
+  const RowLp r = row_lp(logits, stats, s, row, t, pieces);
+  lp[row] = (float)r.lp;
+  saved[row] = make_float4(r.m, r.inv, (float)r.lp, 1.f);
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double sums[kThreads / 64];
+  #pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.;
+  #pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) v += sums[w];
+  return v;
+}
+
+// True in the block that arrives last, once all others' stores to global
+// memory can be read.
+__device__ __forceinline__ bool last_block(unsigned* ticket) {
+  __shared__ bool last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL,
+                                  __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  if (last) __threadfence();
+  return last;
+}
+
+struct PolicyArgs {
+  double low, high;  // bounds of the ratio
+  double kl;
+};
+
+// rho = exp(lp - old);  token loss = -min(rho A, clip(rho) A)
+//                                    + kl (e^d - d - 1),  d = ref - lp
+// The partial sums of the blocks are added in their order by the last one.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void policy_finish_kernel(
+    const T* __restrict__ logits, const long* __restrict__ target,
+    const float2* __restrict__ stats, const float* __restrict__ old_lp,
+    const float* __restrict__ adv, const float* __restrict__ ref_lp,
+    float4* __restrict__ saved, double* __restrict__ partial,
+    unsigned* __restrict__ ticket, float* __restrict__ loss,
+    float* __restrict__ inv_count, Shape s, long ignore, int pieces,
+    PolicyArgs a) {
+  const long row = (long)blockIdx.x * kThreads + threadIdx.x;
+  double tok = 0., count = 0.;
+  if (row < s.rows) {
+    const long t = target[row];
+    float4 keep = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (is_live(t, s.vocab, ignore)) {
+      const RowLp r = row_lp(logits, stats, s, row, t, pieces);
+      const double rho = exp(r.lp - (double)old_lp[row]);
+      const double A = (double)adv[row];
+      const double free = rho * A;
+      const double held = fmin(fmax(rho, a.low), a.high) * A;
+      // the gradient flows where the free term is the smaller one or both
+      // are the same; NaN takes this side as well and stays NaN
+      const bool clipped = free > held;
+      tok = clipped ? -held : -free;
+      double coef = clipped ? 0. : -free;
+      if (ref_lp) {
+        const double d = (double)ref_lp[row] - r.lp;
+        tok += a.kl * (exp(d) - d - 1.);
+        coef += a.kl * (1. - exp(d));
+      }
+      count = 1.;
+      keep = make_float4(r.m, r.inv, (float)r.lp, (float)coef);
+    }
+    saved[row] = keep;
+  }
+  tok = block_sum(tok);
+  count = block_sum(count);
+  if (threadIdx.x == 0) {
+    partial[2 * blockIdx.x] = tok;
+    partial[2 * blockIdx.x + 1] = count;
+  }
+  if (!last_block(ticket)) return;
+  tok = count = 0.;
+  for (unsigned b = threadIdx.x; b < gridDim.x; b += kThreads) {
+    tok += partial[2 * b];
+    count += partial[2 * b + 1];
+  }
+  tok = block_sum(tok);
+  count = block_sum(count);
+  if (threadIdx.x == 0) {
+    const double n = count > 0. ? count : 1.;
+    *loss = (float)(tok / n);
+    *inv_count = (float)(1. / n);
+  }
+}
+
+// One block for each pair: the rewards beta * sum(lp - ref) of its two
+// sequences, h = their difference, and the pair's
+//   loss = (1 - eps) softplus(-h) + eps softplus(h).
+// Rows of the chosen sequence get dl/dlp = beta dl/dh, of the rejected one
+// its negative; the mean over the pairs is in it.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void prefer_finish_kernel(
+    const T* __restrict__ logits, const long* __restrict__ target,
+    const float2* __restrict__ stats, const float* __restrict__ ref_lp,
+    float4* __restrict__ saved, double* __restrict__ partial,
+    unsigned* __restrict__ ticket, float* __restrict__ loss,
+    float* __restrict__ rewards, Shape s, long ignore, int pieces,
+    long seq, double beta, double eps) {
+  const long pairs = gridDim.x, pair = blockIdx.x;
+  double gain[2];
+  for (int side = 0; side < 2; ++side) {
+    const long first = (pair + side * pairs) * seq;
+    double sum = 0.;
+    for (long i = threadIdx.x; i < seq; i += kThreads) {
+      const long row = first + i, t = target[row];
+      float4 keep = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (is_live(t, s.vocab, ignore)) {
+        const RowLp r = row_lp(logits, stats, s, row, t, pieces);
+        sum += r.lp - (double)ref_lp[row];
+        keep = make_float4(r.m, r.inv, (float)r.lp, 0.f);
+      }
+      saved[row] = keep;
+    }
+    gain[side] = beta * block_sum(sum);
+  }
+  const double h = gain[0] - gain[1];
+  const double tail = log1p(exp(-fabs(h)));
+  const double e = exp(-h);  // sigmoid(-h) = e / (1 + e)
+  const double down = h > 0. ? e / (1. + e) : 1. / (1. + exp(h));
+  const double dh = eps - down;  // d loss / d h
+  const float coef = (float)(beta * dh / (double)pairs);
+  for (int side = 0; side < 2; ++side) {
+    const long first = (pair + side * pairs) * seq;
+    for (long i = threadIdx.x; i < seq; i += kThreads) {
+      const long row = first + i;
+      if (is_live(target[row], s.vocab, ignore))
+        saved[row].w = side ? -coef : coef;
+    }
+  }
+  if (threadIdx.x == 0) {
+    rewards[pair] = (float)gain[0];
+    rewards[pair + pairs] = (float)gain[1];
+    partial[pair] = (1. - eps) * (fmax(-h, 0.) + tail) +
+                    eps * (fmax(h, 0.) + tail);
+  }
+  if (!last_block(ticket)) return;
+  double sum = 0.;
+  for (long p = threadIdx.x; p < pairs; p += kThreads) sum += partial[p];
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) *loss = (float)(sum / (double)pairs);
+}
+
+// dx_j = c ([j = t] - exp(x_j - M) / sum),  c = coef * up * scale.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void lp_bwd_kernel(
+    const T* __restrict__ logits, const long* __restrict__ target,
+    const float4* __restrict__ saved, const float* __restrict__ up,
+    int up_step, const float* __restrict__ scale, T* __restrict__ dlogits,
+    Shape s, long ignore, long piece) {
+  const long row = blockIdx.x;
+  const long begin = blockIdx.y * piece;
+  const long end = min(s.vocab, begin + piece);
+  T* dx = dlogits + row * s.vocab;
+  const long t = target[row];
+  const float4 r = saved[row];
+  float c = 0.f;
+  if (is_live(t, s.vocab, ignore)) {
+    c = r.w * up[row * up_step];
+    if (scale) c *= *scale;
+  }
+  if (c == 0.f) {
+    for (long i = begin + threadIdx.x; i < end; i += kThreads)
+      dx[i] = (T)0.f;
+    return;
+  }
+  const T* x = row_of(logits, s, row);
+  const float k = -c * r.y;
+  // 1 - p of a token that is almost certain loses its digits
+  const float at_target = -c * expm1f(r.z);
+  for (long i = begin + threadIdx.x; i < end; i += kThreads) {
+    const float p = __expf((float)x[i] - r.x);
+    dx[i] = (T)(i == t ? at_target : k * p);
+  }
+}
+
+struct Call {
+  Shape s;
+  long ignore;
+  int pieces;
+  long piece;
+};
+
+// Few rows are split over the vocabulary so that the whole chip reads.
+void split(long rows, long vocab, int& pieces, long& piece) {
+  long want = (1024 + rows - 1) / rows;
+  want = std::max<long>(1, std::min<long>(want, (vocab + 4095) / 4096));
+  piece = (vocab + want - 1) / want;
+  pieces = (int)((vocab + piece - 1) / piece);
+}
+
+Call check(const at::Tensor& logits, const at::Tensor& target, long ignore,
+           const char* what) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3 &&
+                  (logits.size(2) <= 1 || logits.stride(2) == 1),
+              what, ": logits [B, S, V] with a unit last stride required");
+  TORCH_CHECK(target.device() == logits.device() &&
+                  target.scalar_type() == at::kLong && target.dim() == 2 &&
+                  target.size(0) == logits.size(0) &&
+                  target.size(1) == logits.size(1) && target.is_contiguous(),
+              what, ": contiguous int64 targets [B, S] required");
+  Call c;
+  c.s = Shape{logits.size(0) * logits.size(1), logits.size(2),
+              std::max<long>(1, logits.size(1)), logits.stride(0),
+              logits.stride(1)};
+  // a launch has fewer than 2^32 threads along x
+  TORCH_CHECK(c.s.rows < (1L << 24) && (c.s.vocab > 0 || c.s.rows == 0),
+              what, ": fewer than 2^24 rows of at least one logit required");
+  c.ignore = ignore;
+  if (c.s.rows > 0) split(c.s.rows, c.s.vocab, c.pieces, c.piece);
+  return c;
+}
+
+void check_rows(const at::Tensor& v, const at::Tensor& target,
+                const char* what) {
+  TORCH_CHECK(v.device() == target.device() && v.is_contiguous() &&
+                  v.scalar_type() == at::kFloat &&
+                  v.sizes() == target.sizes(),
+              what, ": contiguous fp32 values of the targets' shape required");
+}
+
+template <typename T>
+at::Tensor launch_stats(const at::Tensor& logits, const at::Tensor& target,
+                        const Call& c, unsigned* ticket) {
+  auto stats = at::empty({c.s.rows, c.pieces, 2},
+                         logits.options().dtype(at::kFloat));
+  hipLaunchKernelGGL((row_stats_kernel<T>),
+                     dim3((unsigned)c.s.rows, (unsigned)c.pieces),
+                     dim3(kThreads), 0, elem::stream(),
+                     (const T*)logits.data_ptr(), target.data_ptr<long>(),
+                     (float2*)stats.data_ptr(), ticket, c.s, c.ignore,
+                     c.pieces, c.piece);
+  return stats;
+}
+
+}  // namespace
+
+// (lp [B, S] fp32, saved [B, S, 4] fp32)
+std::vector<at::Tensor> token_logprobs_fwd(at::Tensor logits,
+                                           at::Tensor target,
+                                           int64_t ignore) {
+  const Call c = check(logits, target, ignore, "token_logprobs");
+  const c10::DeviceGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  auto lp = at::empty(target.sizes(), f32);
+  auto saved = at::empty({target.size(0), target.size(1), 4}, f32);
+  STOKE_ELEM_SWITCH(logits.scalar_type(), "token_logprobs", {
+    if (c.s.rows > 0) {
+      auto stats = launch_stats<T>(logits, target, c, nullptr);
+      hipLaunchKernelGGL(
+          (lp_finish_kernel<T>),
+          dim3((unsigned)((c.s.rows + kThreads - 1) / kThreads)),
+          dim3(kThreads), 0, elem::stream(), (const T*)logits.data_ptr(),
+          target.data_ptr<long>(), (const float2*)stats.data_ptr(),
+          (float4*)saved.data_ptr(), lp.data_ptr<float>(), c.s, ignore,
+          c.pieces);
+    }
+  });
+  return {lp, saved};
+}
+
+// (loss [], saved [B, S, 4], inv_count [])
+std::vector<at::Tensor> policy_loss_fwd(
+    at::Tensor logits, at::Tensor target, at::Tensor old_lp, at::Tensor adv,
+    c10::optional<at::Tensor> ref_lp, double low, double high, double kl,
+    int64_t ignore) {
+  const Call c = check(logits, target, ignore, "policy_loss");
+  check_rows(old_lp, target, "policy_loss");
+  check_rows(adv, target, "policy_loss");
+  if (ref_lp) check_rows(*ref_lp, target, "policy_loss");
+  const c10::DeviceGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  auto saved = at::empty({target.size(0), target.size(1), 4}, f32);
+  if (c.s.rows == 0)
+    return {at::zeros({}, f32), saved, at::ones({}, f32)};
+  auto loss = at::empty({}, f32), inv_count = at::empty({}, f32);
+  const long blocks = (c.s.rows + kThreads - 1) / kThreads;
+  auto partial = at::empty({2 * blocks + 1}, f32.dtype(at::kDouble));
+  double* part = partial.data_ptr<double>();
+  unsigned* ticket = (unsigned*)(part + 2 * blocks);
+  STOKE_ELEM_SWITCH(logits.scalar_type(), "policy_loss", {
+    auto stats = launch_stats<T>(logits, target, c, ticket);
+    hipLaunchKernelGGL(
+        (policy_finish_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0,
+        elem::stream(), (const T*)logits.data_ptr(),
+        target.data_ptr<long>(), (const float2*)stats.data_ptr(),
+        old_lp.data_ptr<float>(), adv.data_ptr<float>(),
+        ref_lp ? ref_lp->data_ptr<float>() : nullptr,
+        (float4*)saved.data_ptr(), part, ticket, loss.data_ptr<float>(),
+        inv_count.data_ptr<float>(), c.s, ignore, c.pieces,
+        PolicyArgs{low, high, kl});
+  });
+  return {loss, saved, inv_count};
+}
+
+// (loss [], rewards [B], saved [B, S, 4])
+std::vector<at::Tensor> preference_loss_fwd(at::Tensor logits,
+                                            at::Tensor target,
+                                            at::Tensor ref_lp, double beta,
+                                            double eps, int64_t ignore) {
+  const Call c = check(logits, target, ignore, "preference_loss");
+  check_rows(ref_lp, target, "preference_loss");
+  const long pairs = target.size(0) / 2, seq = target.size(1);
+  TORCH_CHECK(pairs > 0 && target.size(0) % 2 == 0,
+              "preference_loss: an even number of sequences required");
+  const c10::DeviceGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  auto saved = at::empty({target.size(0), seq, 4}, f32);
+  auto loss = at::empty({}, f32), rewards = at::empty({2 * pairs}, f32);
+  if (c.s.rows == 0) {
+    loss.fill_(0.6931471805599453);
+    rewards.zero_();
+    return {loss, rewards, saved};
+  }
+  auto partial = at::empty({pairs + 1}, f32.dtype(at::kDouble));
+  double* part = partial.data_ptr<double>();
+  unsigned* ticket = (unsigned*)(part + pairs);
+  STOKE_ELEM_SWITCH(logits.scalar_type(), "preference_loss", {
+    auto stats = launch_stats<T>(logits, target, c, ticket);
+    hipLaunchKernelGGL(
+        (prefer_finish_kernel<T>), dim3((unsigned)pairs), dim3(kThreads), 0,
+        elem::stream(), (const T*)logits.data_ptr(),
+        target.data_ptr<long>(), (const float2*)stats.data_ptr(),
+        ref_lp.data_ptr<float>(), (float4*)saved.data_ptr(), part, ticket,
+        loss.data_ptr<float>(), rewards.data_ptr<float>(), c.s, ignore,
+        c.pieces, seq, beta, eps);
+  });
+  return {loss, rewards, saved};
+}
+
+// up: one value for each row (token_logprobs) or one for all (the losses).
+at::Tensor token_loss_bwd(at::Tensor logits, at::Tensor target,
+                          at::Tensor saved, at::Tensor up,
+                          c10::optional<at::Tensor> scale, int64_t ignore) {
+  const Call c = check(logits, target, ignore, "token_loss");
+  TORCH_CHECK(up.device() == logits.device() && up.is_contiguous() &&
+                  up.scalar_type() == at::kFloat &&
+                  (up.numel() == 1 || up.numel() == c.s.rows),
+              "token_loss: fp32 gradient of one value or one a row required");
+  const c10::DeviceGuard guard(logits.device());
+  auto dlogits = at::empty(logits.sizes(), logits.options());
+  STOKE_ELEM_SWITCH(logits.scalar_type(), "token_loss", {
+    if (c.s.rows > 0)
+      hipLaunchKernelGGL(
+          (lp_bwd_kernel<T>),
+          dim3((unsigned)c.s.rows, (unsigned)c.pieces), dim3(kThreads), 0,
+          elem::stream(), (const T*)logits.data_ptr(),
+          target.data_ptr<long>(), (const float4*)saved.data_ptr(),
+          up.data_ptr<float>(), up.numel() == 1 ? 0 : 1,
+          scale ? scale->data_ptr<float>() : nullptr,
+          (T*)dlogits.data_ptr(), c.s, ignore, c.piece);
+  });
+  return dlogits;
+}

@@ -40,7 +40,8 @@ setup(
                      "csrc/fa_bwd.hip",
                      "csrc/fp8_quant.hip",
                      "csrc/fused_ce.hip",
-                     "csrc/act8.hip"],
+                     "csrc/act8.hip",
+                     "csrc/token_loss.hip"],
             depends=["csrc/elem.h"],
             extra_compile_args={
                 "cxx": ["-O3"],

@@ -12,3 +12,8 @@ from stoke.nn.swiglu import swiglu  # noqa: F401
 from stoke.nn.cross_entropy import fused_cross_entropy  # noqa: F401
 from stoke.nn.attention import attention, flash_attention  # noqa: F401
 from stoke.nn.fp8_delayed import FP8LinearDelayed  # noqa: F401
+from stoke.nn.token_loss import (  # noqa: F401
+    fused_policy_loss,
+    fused_preference_loss,
+    token_logprobs,
+)

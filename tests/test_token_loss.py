@@ -1,0 +1,444 @@
+# -*- coding: utf-8 -*-
+"""Token log-probabilities, policy and preference loss against float64
+formulas (torch path here, HIP kernels in the gpu tier)."""
+
+import pytest
+import torch
+
+from stoke.nn import fused_policy_loss, fused_preference_loss, token_logprobs
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+U = 2.0 ** -24  # half an fp32 step
+IGN = -100
+# one logit, odd and even vocabularies, rows split over blocks and not
+SHAPES = [(1, 1, 1), (1, 1, 2), (2, 3, 7), (2, 5, 255), (4, 3, 1000),
+          (2, 2, 4097), (2, 1, 50257), (6, 200, 129)]
+
+
+def _skip(device):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _inputs(shape, dtype, device, seed=0, keep=0.7):
+    b, s, v = shape
+    g = _gen(seed)
+    x = 3 * torch.randn(b, s, v, generator=g)
+    t = torch.randint(0, v, (b, s), generator=g)
+    x.scatter_add_(-1, t[..., None], 12 * torch.rand(b, s, 1, generator=g))
+    live = torch.rand(b, s, generator=g) < keep
+    live[0, 0] = True
+    if b > 1:
+        live[1] = False  # a sequence without any token
+    t = torch.where(live, t, torch.full_like(t, IGN))
+    return x.to(dtype).to(device), t.to(device)
+
+
+class Oracle:
+    """float64 rows of softmax, lp and how far fp32 sums may be off."""
+
+    def __init__(self, x, t):
+        x, t = x.detach().cpu().double(), t.cpu()
+        v = x.shape[-1]
+        self.live = (t != IGN) & (t >= 0) & (t < v)
+        at = torch.where(self.live, t, torch.zeros_like(t))[..., None]
+        m = x.amax(-1, keepdim=True)
+        d = x - m
+        e = d.exp()
+        z = e.sum(-1, keepdim=True)
+        self.p = e / z
+        lp = (d.gather(-1, at) - z.log())[..., 0]
+        self.lp = torch.where(self.live, lp, torch.zeros_like(lp))
+        self.hot = torch.zeros_like(x).scatter_(-1, at, 1.0)
+        # a term exp(d) is off by 1.25 |d| U (argument of exp2, log2 e) and
+        # 3 U; a thread adds up to v / 256 of them one after another, 80
+        # counts the joins and their factors; with the same again for the
+        # factors' own arguments
+        self.d_u = 1.25 * d.abs().nan_to_num(posinf=0.0) * U
+        far = (self.p * d.abs()).nan_to_num().sum(-1)
+        self.tol_lp = (v / 256 + 80 + 2.5 * far) * U
+
+    def grad(self, c, c_err, dtype, got):
+        """Checks got = c (onehot - p) for row values c known to c_err."""
+        got = got.detach().cpu().double()
+        c_err = torch.where(self.live, c_err, torch.zeros_like(c_err))
+        c = torch.where(self.live, c, torch.zeros_like(c))[..., None]
+        side = self.hot - self.p
+        want = torch.where(self.live[..., None], c * side,
+                           torch.zeros_like(side))
+        slack = (c_err[..., None] + 8 * U * c.abs()) * side.abs() \
+            + c.abs() * self.p * (self.d_u + self.tol_lp[..., None] + 8 * U)
+        fin = torch.finfo(dtype)
+        tol = fin.eps / 2 * (want.abs() + slack) + slack \
+            + fin.tiny * fin.eps / 2
+        bad = (got - want).abs() > torch.where(self.live[..., None], tol,
+                                               torch.zeros_like(tol))
+        assert not bool(bad.any()), (
+            (got - want)[bad][:5], want[bad][:5], int(bad.sum()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_logprobs(shape, dtype, device):
+    _skip(device)
+    x, t = _inputs(shape, dtype, device)
+    x.requires_grad_(True)
+    lp = token_logprobs(x, t)
+    o = Oracle(x, t)
+    assert lp.dtype == torch.float32 and lp.shape == t.shape
+    off = (lp.detach().cpu().double() - o.lp).abs()
+    assert bool((off <= o.tol_lp + U * o.lp.abs()).all())
+    assert bool((lp[~o.live.to(device)] == 0).all())
+    up = torch.randn(t.shape, generator=_gen(5)).to(device)
+    lp.backward(up)
+    o.grad(up.cpu().double(), torch.zeros(t.shape).double(), dtype, x.grad)
+
+
+def _policy_inputs(x, t, seed=1):
+    g, o = _gen(seed), Oracle(x, t)
+    shift = 0.3 * torch.randn(t.shape, generator=g).double()
+    for edge in (0.7, 1.4):  # away from the steps of the gradient
+        at = torch.tensor(edge).double().log()
+        shift = torch.where((shift - at).abs() < 1e-3, shift + 5e-3, shift)
+    old = (o.lp - shift).float()
+    adv = torch.randn(t.shape, generator=g)
+    ref = (o.lp + 0.4 * torch.randn(t.shape, generator=g)).float()
+    return o, old, adv, ref
+
+
+def _policy64(o, old, adv, ref, kl):
+    rho = (o.lp - old.double()).exp()
+    a = adv.double()
+    held = rho.clamp(0.7, 1.4) * a
+    tok = -torch.minimum(rho * a, held)
+    coef = torch.where(rho * a <= held, -rho * a, torch.zeros_like(rho))
+    steep = (rho * a).abs()
+    if kl:
+        d = ref.double() - o.lp
+        tok = tok + kl * (d.exp() - d - 1)
+        coef = coef + kl * (1 - d.exp())
+        steep = steep + kl * (1 + d.exp())
+    n = max(1, int(o.live.sum()))
+    return tok[o.live].sum() / n, coef / n, steep / n, tok
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kl", [0.0, 0.3])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_policy(shape, kl, dtype, device):
+    _skip(device)
+    x, t = _inputs(shape, dtype, device)
+    o, old, adv, ref = _policy_inputs(x, t)
+    x.requires_grad_(True)
+    loss = fused_policy_loss(
+        x, t, old.to(device), adv.to(device),
+        ref_logprobs=ref.to(device) if kl else None, clip_low=0.3,
+        clip_high=0.4, kl_coef=kl)
+    want, coef, steep, tok = _policy64(o, old, adv, ref, kl)
+    assert loss.dtype == torch.float32 and loss.dim() == 0
+    tol = (steep * o.tol_lp)[o.live].sum() + 2 * U * want.abs()
+    assert abs(float(loss.detach()) - float(want)) <= float(tol)
+    loss.backward(torch.tensor(3.0, device=device))
+    o.grad(3 * coef, 3 * steep * o.tol_lp, dtype, x.grad)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("smooth", [0.0, 0.2])
+@pytest.mark.parametrize(
+    "shape", [(2, 1, 1), (2, 3, 7), (4, 5, 255), (2, 2, 4097), (2, 1, 50257),
+              (6, 200, 129), (4, 700, 40)])
+def test_preference(shape, smooth, dtype, device):
+    _skip(device)
+    x, t = _inputs(shape, dtype, device)
+    o = Oracle(x, t)
+    ref = (o.lp + 0.5 * torch.randn(t.shape, generator=_gen(3))).float()
+    x.requires_grad_(True)
+    loss, rewards = fused_preference_loss(
+        x, t, ref.to(device), beta=0.3, label_smoothing=smooth)
+    assert rewards.shape == (shape[0],) and not rewards.requires_grad
+    gap = torch.where(o.live, o.lp - ref.double(),
+                      torch.zeros_like(o.lp)).sum(-1) * 0.3
+    half = shape[0] // 2
+    h = gap[:half] - gap[half:]
+    down, upw = 1 / (1 + h.exp()), 1 / (1 + (-h).exp())
+    want = (-(1 - smooth) * upw.log() - smooth * down.log()).mean()
+    err = 0.3 * torch.where(o.live, o.tol_lp,
+                            torch.zeros_like(o.lp)).sum(-1)
+    off = (rewards.cpu().double() - gap).abs()
+    assert bool((off <= err + 2 * U * gap.abs()).all())
+    assert abs(float(loss) - float(want)) <= float(
+        err.sum() / half + 2 * U * want.abs())
+    loss.backward(torch.tensor(2.0, device=device))
+    dh = 2 * 0.3 / half * (smooth - down)
+    dh_err = 2 * 0.3 / half * 0.25 * (err[:half] + err[half:]) \
+        + 4 * U * dh.abs()
+    c = torch.cat((dh, -dh))[:, None].expand(t.shape)
+    c_err = torch.cat((dh_err, dh_err))[:, None].expand(t.shape)
+    o.grad(c, c_err, dtype, x.grad)
+
+
+# ------------------------------------------------------------------- edges
+@pytest.mark.parametrize("device", DEVICES)
+def test_ignored_rows_are_left_out_whatever_they_hold(device):
+    _skip(device)
+    x, t = _inputs((4, 6, 300), torch.bfloat16, device, keep=1.0)
+    t[0, 2], t[2, 3], t[3, 5] = IGN, 300, -7
+    bad = torch.zeros(4, 6, dtype=torch.bool, device=device)
+    bad[0, 2] = bad[2, 3] = bad[3, 5] = bad[1] = True
+    x[bad] = float("nan")
+    x[0, 2, 5] = float("inf")
+    vals = torch.randn(4, 6, generator=_gen(0)).to(device)
+    vals[bad] = float("nan")
+    up = torch.ones(4, 6, device=device)
+    for fn in (
+        lambda y: (token_logprobs(y, t) * up).sum(),
+        lambda y: fused_policy_loss(y, t, vals, vals, ref_logprobs=vals,
+                                    kl_coef=0.1),
+        lambda y: fused_preference_loss(y, t, vals)[0],
+    ):
+        y = x.clone().requires_grad_(True)
+        loss = fn(y)
+        loss.backward()
+        assert torch.isfinite(loss)
+        assert torch.isfinite(y.grad).all()
+        assert bool((y.grad[bad] == 0).all())
+        assert bool((y.grad[~bad] != 0).any())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_token_left(device):
+    _skip(device)
+    x = torch.randn(2, 3, 10, device=device, requires_grad=True)
+    t = torch.full((2, 3), IGN, device=device)
+    v = torch.zeros(2, 3, device=device)
+    assert float(fused_policy_loss(x, t, v, v)) == 0.0
+    loss, rewards = fused_preference_loss(x, t, v)
+    assert abs(float(loss) - 0.6931471805599453) < 1e-7
+    assert rewards.tolist() == [0.0, 0.0]
+    (fused_policy_loss(x, t, v, v) + loss).backward()
+    assert bool((x.grad == 0).all())
+    e = torch.empty(2, 0, 10, device=device, requires_grad=True)
+    te, ve = t[:, :0], v[:, :0]
+    assert token_logprobs(e, te).shape == (2, 0)
+    assert float(fused_policy_loss(e, te, ve, ve)) == 0.0
+    fused_preference_loss(e, te, ve)[0].backward()
+    assert e.grad.shape == e.shape
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_vocabulary_and_lowest_values(dtype, device):
+    _skip(device)
+    fin = torch.finfo(dtype)
+    x = torch.randn(1, 5, 600, generator=_gen(4)).to(dtype)
+    x[0, 0, 10:] = -float("inf")  # a constrained step
+    x[0, 1, 1:] = fin.min  # masked by the type's lowest value
+    x[0, 2] = -float("inf")
+    x[0, 2, 7] = 3.0  # one token left
+    x[0, 3] = fin.min  # all equal
+    x[0, 4, :300] = fin.max
+    t = torch.tensor([[3, 0, 7, 5, 1]])
+    x, t = x.to(device).requires_grad_(True), t.to(device)
+    lp = token_logprobs(x, t)
+    o = Oracle(x, t)
+    assert torch.isfinite(lp).all()
+    off = (lp.detach().cpu().double() - o.lp).abs()
+    assert bool((off <= o.tol_lp + U * o.lp.abs()).all())
+    lp.sum().backward()
+    assert torch.isfinite(x.grad).all()
+    assert bool((x.grad[0, 0, 10:] == 0).all())
+    assert bool((x.grad[0, 2] == 0).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_without_a_distribution_are_nan(device):
+    _skip(device)
+    x = torch.zeros(1, 4, 500)
+    x[0, 0] = -float("inf")
+    x[0, 1, 3] = float("inf")
+    x[0, 2, 400] = float("nan")
+    t = torch.tensor([[1, 3, 0, 0]], device=device)
+    x = x.to(device).requires_grad_(True)
+    lp = token_logprobs(x, t)
+    assert torch.isnan(lp[0, :3]).all() and torch.isfinite(lp[0, 3])
+    lp.sum().backward()
+    assert torch.isnan(x.grad[0, 2]).any()
+    assert torch.isfinite(x.grad[0, 3]).all()
+    v = torch.zeros(1, 4, device=device)
+    assert torch.isnan(fused_policy_loss(x, t, v, v + 1.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ratio_on_the_clip_and_beyond(device):
+    _skip(device)
+    # uniform over 4 tokens: lp = -log 4; rho = 1/2, 1, 2 with clip [1/2, 2]
+    x = torch.zeros(1, 4, 4, device=device, requires_grad=True)
+    t = torch.zeros(1, 4, dtype=torch.int64, device=device)
+    lp = -torch.tensor(4.0).double().log()
+    old = torch.stack((lp, lp, lp + 2, lp - 2)).float()[None].to(device)
+    adv = torch.tensor([[1.0, -1.0, -1.0, 1.0]], device=device)
+    loss = fused_policy_loss(x, t, old, adv, clip_low=0.5, clip_high=1.0)
+    # rho = 1: -A each; rho = e^-2, A < 0: held at 0.5; rho = e^2, A > 0: at 2
+    assert abs(float(loss) - (-1 + 1 + 0.5 - 2) / 4) < 1e-6
+    loss.backward()
+    g = x.grad[0]
+    assert bool((g[2:] == 0).all())
+    assert abs(float(g[0, 0]) + 0.75 / 4) < 1e-6
+    assert abs(float(g[1, 0]) - 0.75 / 4) < 1e-6
+    # no clip at all: rho stays on it, and the gradient flows
+    x.grad = None
+    old = torch.full((1, 4), float(x[0].log_softmax(-1)[0, 0]), device=device)
+    fused_policy_loss(x, t, old, adv, clip_low=1.0, clip_high=0.0,
+                      ).backward()
+    assert bool((x.grad[0, 1] != 0).any())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layouts_and_broadcast_values(device):
+    _skip(device)
+    x, t = _inputs((2, 9, 101), torch.bfloat16, device, keep=1.0)
+    o, old, adv, ref = _policy_inputs(x, t)
+    old, adv = old.to(device), adv[:, :1].contiguous().to(device)
+    want = token_logprobs(x, t)
+    wide = torch.zeros(2, 11, 130, dtype=x.dtype, device=device)
+    wide[:, 1:10, 3:104] = x
+    view = wide[:, 1:10, 3:104]  # rows at another alignment and stride
+    turned = x.transpose(0, 1).contiguous().transpose(0, 1)
+    last = x.transpose(1, 2).contiguous().transpose(1, 2)  # stride(-1) != 1
+    for y in (view, turned, last):
+        y = y.detach().requires_grad_(True)
+        assert torch.equal(token_logprobs(y, t), want)
+        z = x.clone().requires_grad_(True)
+        a = fused_policy_loss(y, t, old, adv)
+        b = fused_policy_loss(z, t, old, adv.expand(2, 9).clone())
+        assert torch.equal(a, b)
+        ga, = torch.autograd.grad(a, y)
+        gb, = torch.autograd.grad(b, z)
+        assert torch.equal(ga, gb)
+    assert torch.equal(token_logprobs(x[0], t[0]), want[0])
+    assert torch.equal(token_logprobs(x[None], t[None]), want[None])
+    assert torch.equal(
+        token_logprobs(x[:, :-1], t[:, 1:].contiguous() * 0), token_logprobs(
+            x, torch.zeros_like(t))[:, :-1])
+    flat = fused_policy_loss(x.flatten(0, 1), t.flatten(), old.flatten(),
+                             adv.expand(2, 9).flatten())
+    # another split of the same float64 sum over the tokens
+    assert abs(float(flat) - float(fused_policy_loss(x, t, old, adv))) \
+        <= 4 * U * abs(float(flat)) + 1e-12
+
+
+def test_gradients_against_differences():
+    x, t = _inputs((4, 3, 11), torch.float32, "cpu", keep=1.0)
+    x = x.double()
+    o, old, adv, ref = _policy_inputs(x, t)
+    old, adv, ref = old.double(), adv.double(), ref.double()
+    for fn in (
+        lambda y: fused_policy_loss(y, t, old, adv, ref, 0.3, 0.4, 0.2),
+        lambda y: fused_preference_loss(y, t, ref, 0.3, 0.1)[0],
+        lambda y: (token_logprobs(y, t) * adv).sum(),
+    ):
+        assert torch.autograd.gradcheck(fn, (x.requires_grad_(True),))
+
+
+def test_refusals():
+    x, t = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64)
+    v = torch.zeros(2, 3)
+    cases = [
+        lambda: token_logprobs(x, t.int()),
+        lambda: token_logprobs(x, t[:, :2]),
+        lambda: token_logprobs(x[0, 0], t[0, 0]),
+        lambda: token_logprobs(x.long(), t),
+        lambda: token_logprobs(x[..., :0], t),
+        lambda: fused_policy_loss(x, t, v[:, :2], v),
+        lambda: fused_policy_loss(x, t, v, v[0]),
+        lambda: fused_policy_loss(x, t, v.long(), v),
+        lambda: fused_policy_loss(x, t, v.clone().requires_grad_(True), v),
+        lambda: fused_policy_loss(x, t, v, v, kl_coef=0.1),
+        lambda: fused_policy_loss(x, t, v, v, v, kl_coef=-0.1),
+        lambda: fused_policy_loss(x, t, v, v, clip_low=1.5),
+        lambda: fused_policy_loss(x, t, v, v, clip_high=-0.1),
+        lambda: fused_preference_loss(x[:1], t[:1], v[:1]),
+        lambda: fused_preference_loss(x[0], t[0], v[0]),
+        lambda: fused_preference_loss(x[:0], t[:0], v[:0]),
+        lambda: fused_preference_loss(x, t, v, beta=0.0),
+        lambda: fused_preference_loss(x, t, v, label_smoothing=0.6),
+        lambda: fused_preference_loss(x, t, v[:, :2]),
+    ]
+    for call in cases:
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.gpu
+def test_gpu_results_repeat_bit_for_bit():
+    _skip("cuda")
+    x, t = _inputs((4, 300, 5000), torch.bfloat16, "cuda", keep=1.0)
+    o, old, adv, ref = _policy_inputs(x, t)
+    old, adv, ref = old.cuda(), adv.cuda(), ref.cuda()
+    first = None
+    for _ in range(3):
+        y = x.clone().requires_grad_(True)
+        a = fused_policy_loss(y, t, old, adv, ref, kl_coef=0.1)
+        b, r = fused_preference_loss(y, t, ref)
+        g, = torch.autograd.grad(a + b, y)
+        now = (a.detach(), b.detach(), r, g)
+        first = first or now
+        assert all(torch.equal(p, q) for p, q in zip(first, now))
+
+
+@pytest.mark.gpu
+def test_gpu_losses_replay_in_a_graph():
+    _skip("cuda")
+    x, t = _inputs((4, 70, 777), torch.bfloat16, "cuda", keep=1.0)
+    o, old, adv, ref = _policy_inputs(x, t)
+    old, adv, ref = old.cuda(), adv.cuda(), ref.cuda()
+    logits = x.clone().requires_grad_(True)
+
+    def step():
+        a = fused_policy_loss(logits, t, old, adv, ref, kl_coef=0.1)
+        b, r = fused_preference_loss(logits, t, ref)
+        return (a.detach(), b.detach(), r,
+                *torch.autograd.grad((a, b), logits))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            logits.copy_(x * (1 + 0.1 * i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in out]
+        want = step()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), i
+
+
+@pytest.mark.gpu
+def test_gpu_on_another_stream():
+    _skip("cuda")
+    x, t = _inputs((2, 40, 3001), torch.bfloat16, "cuda", keep=1.0)
+    want = token_logprobs(x, t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = x.clone().requires_grad_(True)
+        lp = token_logprobs(y, t)
+        g, = torch.autograd.grad(lp.sum(), y)
+    side.synchronize()
+    assert torch.equal(lp, want)
+    z = x.clone().requires_grad_(True)
+    gz, = torch.autograd.grad(token_logprobs(z, t).sum(), z)
+    assert torch.equal(g, gz)
