@@ -712,6 +712,18 @@ at::Tensor token_loss_bwd(at::Tensor logits, at::Tensor target,
                           at::Tensor saved, at::Tensor up,
                           c10::optional<at::Tensor> scale, int64_t ignore);
 
+// Norm and rotation of query and key heads (csrc/qk_norm_rope.hip)
+std::vector<at::Tensor> qk_norm_rope_fwd(
+    at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq,
+    c10::optional<at::Tensor> wk, at::Tensor cosines, at::Tensor sines,
+    c10::optional<at::Tensor> pos, std::vector<int64_t> sections, double eps,
+    bool interleaved);
+std::vector<at::Tensor> qk_norm_rope_bwd(
+    at::Tensor dyq, at::Tensor dyk, at::Tensor q, at::Tensor k,
+    c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
+    at::Tensor cosines, at::Tensor sines, c10::optional<at::Tensor> pos,
+    std::vector<int64_t> sections, double eps, bool interleaved);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &ce_fwd, "fused bf16 cross-entropy forward (online lse)");
   m.def("ce_bwd", &ce_bwd, "fused bf16 cross-entropy backward");
@@ -772,5 +784,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "paired preference loss, forward");
   m.def("token_loss_bwd", &token_loss_bwd,
         "logits' gradient of a loss on token log-probabilities");
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd,
+        "per-head RMS norm and rotation of queries and keys");
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd,
+        "gradients of the heads and weights of qk_norm_rope");
   m.attr("_built_for") = "gfx950";
 }

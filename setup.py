@@ -41,7 +41,8 @@ setup(
                      "csrc/fp8_quant.hip",
                      "csrc/fused_ce.hip",
                      "csrc/act8.hip",
-                     "csrc/token_loss.hip"],
+                     "csrc/token_loss.hip",
+                     "csrc/qk_norm_rope.hip"],
             depends=["csrc/elem.h"],
             extra_compile_args={
                 "cxx": ["-O3"],

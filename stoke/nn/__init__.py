@@ -17,3 +17,4 @@ from stoke.nn.token_loss import (  # noqa: F401
     fused_preference_loss,
     token_logprobs,
 )
+from stoke.nn.qk_norm import StokeQKNorm, qk_norm_rope  # noqa: F401
