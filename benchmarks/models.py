@@ -215,8 +215,13 @@ from stoke.nn.rope import apply_rope  # noqa: E402
 
 
 class LlamaBlock(nn.Module):
-    def __init__(self, d, nh, nkv, ffn):
+    """qk_norm: normalise every query and key head before the rotation.
+    act_bits=8: the MLP's gate and up wait for the backward in 8 bits."""
+
+    def __init__(self, d, nh, nkv, ffn, qk_norm=False, act_bits=16):
         super().__init__()
+        from stoke.nn import StokeQKNorm
+
         self.nh, self.nkv = nh, nkv
         self.hd = d // nh
         self.attn_norm = RMSNorm(d)
@@ -224,6 +229,8 @@ class LlamaBlock(nn.Module):
         self.wk = nn.Linear(d, nkv * self.hd, bias=False)
         self.wv = nn.Linear(d, nkv * self.hd, bias=False)
         self.wo = nn.Linear(nh * self.hd, d, bias=False)
+        self.qk_norm = StokeQKNorm(self.hd) if qk_norm else None
+        self.act_bits = act_bits
         self.mlp_norm = RMSNorm(d)
         self.w_gate = nn.Linear(d, ffn, bias=False)
         self.w_up = nn.Linear(d, ffn, bias=False)
@@ -233,9 +240,14 @@ class LlamaBlock(nn.Module):
         B, S, D = x.shape
         h = self.attn_norm(x)
         # RoPE on the contiguous [B, S, H, Dh] projections (one fused kernel
-        # each), then the attention transpose
-        q = apply_rope(self.wq(h).view(B, S, self.nh, self.hd), cos, sin)
-        k = apply_rope(self.wk(h).view(B, S, self.nkv, self.hd), cos, sin)
+        # each, or one for both with the head norm), then the attention
+        # transpose
+        q = self.wq(h).view(B, S, self.nh, self.hd)
+        k = self.wk(h).view(B, S, self.nkv, self.hd)
+        if self.qk_norm is not None:
+            q, k = self.qk_norm(q, k, cos, sin)
+        else:
+            q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         q = q.transpose(1, 2)
         k = k.transpose(1, 2)
         v = self.wv(h).view(B, S, self.nkv, self.hd).transpose(1, 2)
@@ -247,7 +259,9 @@ class LlamaBlock(nn.Module):
         h = self.mlp_norm(x)
         from stoke.nn import swiglu
 
-        return x + self.w_down(swiglu(self.w_gate(h), self.w_up(h)))
+        return x + self.w_down(
+            swiglu(self.w_gate(h), self.w_up(h), save_bits=self.act_bits)
+        )
 
 
 class Llama(nn.Module):
@@ -262,11 +276,14 @@ class Llama(nn.Module):
         nkv=8,
         ffn=14336,
         max_seq=8192,
+        qk_norm=False,
+        act_bits=16,
     ):
         super().__init__()
         self.embed = nn.Embedding(vocab, d)
         self.blocks = nn.ModuleList(
-            [LlamaBlock(d, nh, nkv, ffn) for _ in range(nlayer)]
+            [LlamaBlock(d, nh, nkv, ffn, qk_norm=qk_norm, act_bits=act_bits)
+             for _ in range(nlayer)]
         )
         self.norm = RMSNorm(d)
         self.head = nn.Linear(d, vocab, bias=False)
@@ -290,7 +307,8 @@ def llama3_8b(vocab=128256, max_seq=8192):
                  max_seq=max_seq)
 
 
-def llama_tiny(vocab=1024, d=256, nlayer=2, nh=4, nkv=2, ffn=512):
+def llama_tiny(vocab=1024, d=256, nlayer=2, nh=4, nkv=2, ffn=512,
+               qk_norm=False, act_bits=16):
     """Small shape for CPU tests."""
     return Llama(vocab=vocab, d=d, nlayer=nlayer, nh=nh, nkv=nkv, ffn=ffn,
-                 max_seq=512)
+                 max_seq=512, qk_norm=qk_norm, act_bits=act_bits)

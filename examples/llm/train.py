@@ -90,15 +90,22 @@ def main():
     ap.add_argument("--buckets", type=int, default=4)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--act-ckpt", action="store_true")
+    ap.add_argument("--act-bits", type=int, default=16, choices=(16, 8),
+                    help="bits of the activations that wait for the "
+                         "backward: checkpoints and SwiGLU inputs")
+    ap.add_argument("--qk-norm", action="store_true",
+                    help="normalise query and key heads before the rotation")
     args = ap.parse_args()
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
     distributed = world > 1
     nh = max(4, args.dim // 128)
     model = Llama(vocab=args.vocab, d=args.dim, nlayer=args.layers, nh=nh,
-                  nkv=max(2, nh // 2), ffn=2 * args.dim, max_seq=512)
+                  nkv=max(2, nh // 2), ffn=2 * args.dim, max_seq=512,
+                  qk_norm=args.qk_norm, act_bits=args.act_bits)
     if args.act_ckpt:
-        apply_activation_checkpointing(model, min_params=10_000)
+        apply_activation_checkpointing(model, min_params=10_000,
+                                       save_bits=args.act_bits)
 
     s = Stoke(
         model=model,

@@ -1,0 +1,135 @@
+# -*- coding: utf-8 -*-
+"""The fine-tuning operators together, as a step uses them: scoring, policy
+and preference losses over a decoder with normalised heads, 8-bit SwiGLU
+inputs and 8-bit checkpoints."""
+
+import os
+import subprocess
+import sys
+from contextlib import nullcontext
+
+import pytest
+import torch
+
+from benchmarks.models import LlamaBlock, llama_tiny
+from stoke.nn import (
+    apply_activation_checkpointing,
+    fused_policy_loss,
+    fused_preference_loss,
+    token_logprobs,
+)
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _skip(device):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def _model(bits, device, dtype, ckpt=True):
+    torch.manual_seed(0)
+    m = llama_tiny(qk_norm=True, act_bits=bits).to(device=device, dtype=dtype)
+    if ckpt:
+        n = apply_activation_checkpointing(
+            m, predicate=lambda _, x: isinstance(x, LlamaBlock),
+            save_bits=bits)
+        assert n == 2
+    return m.train()
+
+
+def _batch(device):
+    g = torch.Generator().manual_seed(7)
+    x = torch.randint(0, 1024, (4, 33), generator=g)
+    y = x[:, 1:].clone()
+    y[:, :5] = -100  # prompts
+    y[2, 20:] = -100  # a padded answer
+    return x[:, :-1].to(device), y.to(device)
+
+
+def _step(m, x, y, amp=nullcontext):
+    # a region for each forward, as the facade has it: autocast keeps its
+    # weight casts until the region ends, and those made without gradient
+    # must not serve a forward that needs one
+    with torch.no_grad(), amp():
+        old = token_logprobs(m(x), y)
+    ref = old - 0.05
+    adv = torch.tensor([[1.0], [-0.5], [0.3], [-1.0]], device=x.device)
+    with amp():
+        logits = m(x)
+    a = fused_policy_loss(logits, y, old, adv, ref_logprobs=ref, kl_coef=0.1)
+    b, rewards = fused_preference_loss(logits, y, ref, beta=0.2)
+    params = dict(m.named_parameters())
+    grads = torch.autograd.grad(a + b, list(params.values()))
+    return a.detach(), b.detach(), rewards, dict(zip(params, grads))
+
+
+def test_step_on_the_cpu():
+    x, y = _batch("cpu")
+    plain = _step(_model(16, "cpu", torch.float32, ckpt=False), x, y)
+    ck16 = _step(_model(16, "cpu", torch.float32), x, y)
+    held = _step(_model(8, "cpu", torch.float32), x, y)
+    assert any("qk_norm.q_weight" in n for n in plain[3])
+    # with the policy that sampled, rho is 1: loss = -mean(A over tokens)
+    n = (y >= 0).sum(-1).double()
+    adv = torch.tensor([1.0, -0.5, 0.3, -1.0]).double()
+    kl = 0.1 * (torch.tensor(-0.05).double().exp() + 0.05 - 1)
+    want = -(adv * n).sum() / n.sum() + kl
+    for loss, pref, rewards, grads in (plain, ck16, held):
+        # lp of the two passes agree to fp32; so does the ratio to 1
+        assert abs(float(loss) - float(want)) < 1e-5
+        assert torch.allclose(rewards.double(), 0.2 * 0.05 * n, atol=1e-4)
+    for name, g in plain[3].items():
+        assert torch.allclose(ck16[3][name], g, atol=1e-6, rtol=1e-4), name
+        off = float((held[3][name] - g).norm() / g.norm())
+        assert off < 0.1, (name, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 8])
+def test_gpu_step_follows_the_cpu(bits):
+    _skip("cuda")
+    # fp32 runs the same kernels for norm, SwiGLU, checkpoints and losses;
+    # only the products differ from the CPU's
+    a = _step(_model(bits, "cpu", torch.float32), *_batch("cpu"))
+    b = _step(_model(bits, "cuda", torch.float32), *_batch("cuda"))
+    assert abs(float(a[0]) - float(b[0])) < 1e-4
+    assert abs(float(a[1]) - float(b[1])) < 1e-4
+    for name, g in a[3].items():
+        off = float((b[3][name].cpu() - g).norm() / g.norm())
+        # a value near the middle of two 8-bit steps may go to the other one
+        assert off < (1e-3 if bits == 16 else 2e-2), (name, off)
+
+
+@pytest.mark.gpu
+def test_gpu_step_under_autocast_and_in_bf16():
+    _skip("cuda")
+    want = _step(_model(16, "cpu", torch.float32), *_batch("cpu"))
+    x, y = _batch("cuda")
+    m = _model(8, "cuda", torch.float32)
+    auto = _step(m, x, y, lambda: torch.autocast("cuda", torch.bfloat16))
+    half = _step(_model(8, "cuda", torch.bfloat16), x, y)
+    for got in (auto, half):
+        assert abs(float(got[0]) - float(want[0])) < 0.05
+        for name, g in got[3].items():
+            assert torch.isfinite(g).all(), name
+            w = want[3][name]
+            cos = torch.nn.functional.cosine_similarity(
+                g.float().cpu().flatten(), w.flatten(), dim=0)
+            assert float(cos) > 0.9, (name, float(cos))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_example_runs(device):
+    _skip(device)
+    cmd = [sys.executable, os.path.join(REPO, "examples", "llm", "train.py"),
+           "--layers", "2", "--dim", "256", "--steps", "2", "--batch", "4",
+           "--act-ckpt", "--act-bits", "8", "--qk-norm"]
+    if device == "cpu":
+        cmd.append("--cpu")
+    env = {k: v for k, v in os.environ.items() if k != "WORLD_SIZE"}
+    r = subprocess.run(cmd, cwd=REPO, env=env, capture_output=True,
+                       text=True, timeout=110)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+    assert "done: 2 steps" in r.stdout
