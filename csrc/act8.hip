@@ -15,8 +15,6 @@
 
 namespace {
 
-using elem::kVec;
-
 // E for a block whose largest magnitude has these fp32 bits.
 __device__ __forceinline__ unsigned block_exponent(unsigned top) {
   const int be = (int)(top >> 23);
@@ -59,16 +57,107 @@ __device__ __forceinline__ unsigned half_wave_max(unsigned v) {
 }
 
 constexpr int kThreads = 256;
+constexpr int kRun = 8;  // values of a thread: 4 threads hold a block of 32
 
-// One value per lane: any length.
+template <typename T>
+using Run = elem::vec<T, kRun>;
+using Bytes = elem::vec<signed char, kRun>;
+
+// Largest over the 4 lanes of a quad, which hold one block.
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 15, 15, true));
+  return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 15, 15,
+                                                   true));
+}
+
+// A quad's block: its exponent, and the thread's 8 values in 8 bits.
+__device__ __forceinline__ unsigned pack_run(const float (&v)[kRun],
+                                             Bytes& q) {
+  unsigned top = 0;
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e)
+    top = max(top, __float_as_uint(v[e]) & 0x7fffffff);
+  const unsigned exp = block_exponent(quad_max(top));
+  // adding 1.5 * 2^23 leaves the whole number, half to even, in the low
+  // bits: its lowest byte is the signed byte
+  const float inv = pow2_bits(254 - exp);
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e)
+    q[e] = (signed char)__float_as_uint(
+        __builtin_fmaf(v[e], inv, 12582912.f));
+  if (exp == 255) q = (Bytes)(signed char)0;
+  return exp;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_run(const Bytes q, unsigned exp,
+                                           float (&v)[kRun]) {
+  const float step = pow2_bits(exp);  // inf for 255: 0 * inf = NaN
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e) v[e] = (float)q[e] * step;
+  // only the topmost exponents can pass the largest value
+  constexpr unsigned kTop = sizeof(T) == 2 && std::is_same_v<T, _Float16>
+                                ? 127 + 10 : 127 + 122;
+  if (exp >= kTop) {
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) v[e] = restored<T>(q[e], exp);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_run(const T* __restrict__ p, long i,
+                                         float (&v)[kRun]) {
+  const Run<T> w = *(const Run<T>*)(p + i);
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e) v[e] = (float)w[e];
+}
+
+template <typename T>
+__device__ __forceinline__ void store_run(T* __restrict__ p, long i,
+                                          const float (&v)[kRun]) {
+  Run<T> w;
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e) w[e] = (T)v[e];
+  *(Run<T>*)(p + i) = w;
+}
+
+__device__ __forceinline__ float sigmoid(float a) {
+  return 1.f / (1.f + __expf(-a));
+}
+
+// y = silu(g) u
+__device__ __forceinline__ float swiglu(float a, float b) {
+  return a / (1.f + __expf(-a)) * b;
+}
+
+// dg = dy u s (1 + g (1 - s)),  du = dy g s,  s = 1 / (1 + e^-g)
+__device__ __forceinline__ void swiglu_grad(float d, float a, float b,
+                                            float& da, float& db) {
+  const float s = sigmoid(a);
+  da = d * b * s * (1.f + a * (1.f - s));
+  db = d * a * s;
+}
+
+// Every kernel has two forms.  The first takes 8 values a thread, with 16-byte (or
+// two 16-byte) accesses for the whole blocks of 32; the last, partial block
+// and tensors that do not start on 16 bytes go one value a thread.  `first`
+// is where the second form begins, a multiple of 32.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pack_kernel(
     const T* __restrict__ x, signed char* __restrict__ q,
-    unsigned char* __restrict__ scale, long n) {
+    unsigned char* __restrict__ scale, long n, long first) {
   const long step = (long)gridDim.x * kThreads;
+  const long me = (long)blockIdx.x * kThreads + threadIdx.x;
+  for (long i = me * kRun; i < first; i += step * kRun) {
+    float v[kRun];
+    Bytes b;
+    load_run(x, i, v);
+    const unsigned e = pack_run(v, b);
+    *(Bytes*)(q + i) = b;
+    if ((threadIdx.x & 3) == 0) scale[i >> 5] = (unsigned char)e;
+  }
   const long n32 = (n + 31) / 32 * 32;
-  for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < n32;
-       i += step) {
+  for (long i = first + me; i < n32; i += step) {
     const float v = i < n ? (float)x[i] : 0.f;
     const unsigned e =
         block_exponent(half_wave_max(__float_as_uint(v) & 0x7fffffff));
@@ -80,9 +169,16 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(
 template <typename T>
 __global__ __launch_bounds__(kThreads) void unpack_kernel(
     const signed char* __restrict__ q,
-    const unsigned char* __restrict__ scale, T* __restrict__ x, long n) {
+    const unsigned char* __restrict__ scale, T* __restrict__ x, long n,
+    long first) {
   const long step = (long)gridDim.x * kThreads;
-  for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < n; i += step)
+  const long me = (long)blockIdx.x * kThreads + threadIdx.x;
+  for (long i = me * kRun; i < first; i += step * kRun) {
+    float v[kRun];
+    unpack_run<T>(*(const Bytes*)(q + i), scale[i >> 5], v);
+    store_run(x, i, v);
+  }
+  for (long i = first + me; i < n; i += step)
     x[i] = (T)restored<T>(q[i], scale[i >> 5]);
 }
 
@@ -91,11 +187,28 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     const T* __restrict__ g, const T* __restrict__ u, T* __restrict__ y,
     signed char* __restrict__ qg, signed char* __restrict__ qu,
-    unsigned char* __restrict__ sg, unsigned char* __restrict__ su, long n) {
+    unsigned char* __restrict__ sg, unsigned char* __restrict__ su, long n,
+    long first) {
   const long step = (long)gridDim.x * kThreads;
+  const long me = (long)blockIdx.x * kThreads + threadIdx.x;
+  for (long i = me * kRun; i < first; i += step * kRun) {
+    float a[kRun], b[kRun], o[kRun];
+    load_run(g, i, a);
+    load_run(u, i, b);
+    Bytes qa, qb;
+    const unsigned ea = pack_run(a, qa), eb = pack_run(b, qb);
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) o[e] = swiglu(a[e], b[e]);
+    store_run(y, i, o);
+    *(Bytes*)(qg + i) = qa;
+    *(Bytes*)(qu + i) = qb;
+    if ((threadIdx.x & 3) == 0) {
+      sg[i >> 5] = (unsigned char)ea;
+      su[i >> 5] = (unsigned char)eb;
+    }
+  }
   const long n32 = (n + 31) / 32 * 32;
-  for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < n32;
-       i += step) {
+  for (long i = first + me; i < n32; i += step) {
     const float a = i < n ? (float)g[i] : 0.f;
     const float b = i < n ? (float)u[i] : 0.f;
     const unsigned eg =
@@ -103,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     const unsigned eu =
         block_exponent(half_wave_max(__float_as_uint(b) & 0x7fffffff));
     if (i < n) {
-      y[i] = (T)(a / (1.f + __expf(-a)) * b);
+      y[i] = (T)swiglu(a, b);
       qg[i] = (signed char)quantize(a, eg);
       qu[i] = (signed char)quantize(b, eu);
     }
@@ -114,27 +227,44 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
   }
 }
 
-// dg = dy u s (1 + g (1 - s)),  du = dy g s,  s = 1 / (1 + e^-g)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void swiglu8_bwd_kernel(
     const T* __restrict__ dy, const signed char* __restrict__ qg,
     const signed char* __restrict__ qu, const unsigned char* __restrict__ sg,
     const unsigned char* __restrict__ su, T* __restrict__ dg,
-    T* __restrict__ du, long n) {
+    T* __restrict__ du, long n, long first) {
   const long step = (long)gridDim.x * kThreads;
-  for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
-    const float a = restored<T>(qg[i], sg[i >> 5]);
-    const float b = restored<T>(qu[i], su[i >> 5]);
-    const float d = (float)dy[i];
-    const float s = 1.f / (1.f + __expf(-a));
-    dg[i] = (T)(d * b * s * (1.f + a * (1.f - s)));
-    du[i] = (T)(d * a * s);
+  const long me = (long)blockIdx.x * kThreads + threadIdx.x;
+  for (long i = me * kRun; i < first; i += step * kRun) {
+    float d[kRun], a[kRun], b[kRun], da[kRun], db[kRun];
+    load_run(dy, i, d);
+    unpack_run<T>(*(const Bytes*)(qg + i), sg[i >> 5], a);
+    unpack_run<T>(*(const Bytes*)(qu + i), su[i >> 5], b);
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e)
+      swiglu_grad(d[e], a[e], b[e], da[e], db[e]);
+    store_run(dg, i, da);
+    store_run(du, i, db);
+  }
+  for (long i = first + me; i < n; i += step) {
+    float da, db;
+    swiglu_grad((float)dy[i], restored<T>(qg[i], sg[i >> 5]),
+                restored<T>(qu[i], su[i >> 5]), da, db);
+    dg[i] = (T)da;
+    du[i] = (T)db;
   }
 }
 
-inline dim3 grid_for(long items) {
-  return dim3((unsigned)std::min<long>((items + kThreads - 1) / kThreads,
-                                       65536));
+// Where the form of one value a thread begins.
+template <typename... P>
+long first_of(long n, P... p) {
+  return (elem::aligned16(p) && ...) ? n / 32 * 32 : 0;
+}
+
+inline dim3 grid_for(long n, long first) {
+  const long threads = std::max(first / kRun, n - first);
+  return dim3((unsigned)std::min<long>((threads + kThreads - 1) / kThreads,
+                                       1 << 20));
 }
 
 // Pieces of the byte buffer that holds g and u: both values, then both
@@ -165,11 +295,12 @@ std::vector<at::Tensor> act8_pack(at::Tensor x) {
   auto q = at::empty(x.sizes(), x.options().dtype(at::kChar));
   auto scale = at::empty({(n + 31) / 32}, x.options().dtype(at::kByte));
   STOKE_ELEM_SWITCH(x.scalar_type(), "act8_pack", {
+    const long first = first_of(n, x.data_ptr());
     if (n > 0)
-      hipLaunchKernelGGL((pack_kernel<T>), grid_for(n), dim3(kThreads), 0,
-                         elem::stream(), (const T*)x.data_ptr(),
-                         (signed char*)q.data_ptr(),
-                         (unsigned char*)scale.data_ptr(), n);
+      hipLaunchKernelGGL((pack_kernel<T>), grid_for(n, first),
+                         dim3(kThreads), 0, elem::stream(),
+                         (const T*)x.data_ptr(), (signed char*)q.data_ptr(),
+                         (unsigned char*)scale.data_ptr(), n, first);
   });
   return {q, scale};
 }
@@ -186,11 +317,13 @@ at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype) {
   const c10::DeviceGuard guard(q.device());
   auto x = at::empty(q.sizes(), q.options().dtype(dtype));
   STOKE_ELEM_SWITCH(dtype, "act8_unpack", {
+    const long first = first_of(n, q.data_ptr());
     if (n > 0)
-      hipLaunchKernelGGL((unpack_kernel<T>), grid_for(n), dim3(kThreads), 0,
-                         elem::stream(), (const signed char*)q.data_ptr(),
+      hipLaunchKernelGGL((unpack_kernel<T>), grid_for(n, first),
+                         dim3(kThreads), 0, elem::stream(),
+                         (const signed char*)q.data_ptr(),
                          (const unsigned char*)scale.data_ptr(),
-                         (T*)x.data_ptr(), n);
+                         (T*)x.data_ptr(), n, first);
   });
   return x;
 }
@@ -209,11 +342,12 @@ std::vector<at::Tensor> swiglu8_fwd(at::Tensor g, at::Tensor u) {
                         g.options().dtype(at::kByte));
   const Held h(held.data_ptr(), n);
   STOKE_ELEM_SWITCH(g.scalar_type(), "swiglu8", {
+    const long first = first_of(n, g.data_ptr(), u.data_ptr());
     if (n > 0)
-      hipLaunchKernelGGL((swiglu8_fwd_kernel<T>), grid_for(n),
+      hipLaunchKernelGGL((swiglu8_fwd_kernel<T>), grid_for(n, first),
                          dim3(kThreads), 0, elem::stream(),
                          (const T*)g.data_ptr(), (const T*)u.data_ptr(),
-                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n);
+                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first);
   });
   return {y, held};
 }
@@ -229,11 +363,12 @@ std::vector<at::Tensor> swiglu8_bwd(at::Tensor dy, at::Tensor held) {
   auto dg = at::empty_like(dy);
   auto du = at::empty_like(dy);
   STOKE_ELEM_SWITCH(dy.scalar_type(), "swiglu8", {
+    const long first = first_of(n, dy.data_ptr());
     if (n > 0)
-      hipLaunchKernelGGL((swiglu8_bwd_kernel<T>), grid_for(n),
+      hipLaunchKernelGGL((swiglu8_bwd_kernel<T>), grid_for(n, first),
                          dim3(kThreads), 0, elem::stream(),
                          (const T*)dy.data_ptr(), h.qg, h.qu, h.sg, h.su,
-                         (T*)dg.data_ptr(), (T*)du.data_ptr(), n);
+                         (T*)dg.data_ptr(), (T*)du.data_ptr(), n, first);
   });
   return {dg, du};
 }

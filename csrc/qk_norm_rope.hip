@@ -196,6 +196,355 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
   }
 }
 
+// ---------------------------------------------------------------------------
+// Rows in registers: G lanes hold a row, 8 values each, so a wave works on
+// 64 / G heads of one token at a time and goes through the token's heads of
+// queries, then keys.  The angles and positions of a token are read once.
+// Needs 16-byte rows: D, strides and pairs in multiples of 8 (see fits()).
+constexpr int kRun = 8;
+
+template <typename T>
+using Run = elem::vec<T, kRun>;
+
+template <typename T>
+__device__ __forceinline__ void unpack(const Run<T>& w, float (&v)[kRun]) {
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e) v[e] = (float)w[e];
+}
+
+// The same run of another lane.
+template <typename T>
+__device__ __forceinline__ Run<T> from_lane(const Run<T>& w, int lane) {
+  constexpr int kWords = kRun * sizeof(T) / 4;
+  union { Run<T> run; int word[kWords]; } in, out;
+  in.run = w;
+  #pragma unroll
+  for (int i = 0; i < kWords; ++i)
+    out.word[i] = __builtin_amdgcn_ds_bpermute(lane << 2, in.word[i]);
+  return out.run;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 15, 15, true));
+}
+
+// Sum over the G lanes of a row; every lane gets it.
+template <int G>
+__device__ __forceinline__ float row_sum(float v) {
+  v += dpp<0xB1>(v);                // lane ^ 1
+  v += dpp<0x4E>(v);                // lane ^ 2
+  v += dpp<0x141>(v);               // mirror in 8: the other quad
+  if (G >= 16) v += dpp<0x140>(v);  // mirror in 16: the other 8
+  if (G >= 32) v += __shfl_xor(v, 16);
+  if (G >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
+// What a lane keeps for all rows of a token: pairs are in the lane
+// (interleaved) or in the lane `other` (halves), `sign` is that of the
+// partner's term in the forward rotation.
+struct Lane {
+  int e0, other, p0;
+  bool on, turns;
+  float sign;
+};
+
+template <int G, bool INTER>
+__device__ __forceinline__ Lane lane_of(const Args& a) {
+  const int lane = threadIdx.x & 63, sub = lane % G;
+  Lane l;
+  l.e0 = sub * kRun;
+  l.on = l.e0 < a.dim;
+  l.turns = l.e0 < 2 * a.half;
+  l.other = lane;
+  l.sign = 1.f;
+  if (INTER) {
+    l.p0 = l.e0 / 2;
+  } else {
+    const bool first = l.e0 < a.half;
+    l.p0 = first ? l.e0 : l.e0 - a.half;
+    if (l.turns) l.other = first ? lane + a.half / kRun
+                                 : lane - a.half / kRun;
+    l.sign = first ? -1.f : 1.f;
+  }
+  return l;
+}
+
+// Angles of a lane's pairs at a token (the identity where nothing turns).
+template <bool INTER>
+__device__ __forceinline__ void angles(const Args& a, const Lane& l,
+                                       long token, long in_seq, float* c,
+                                       float* s) {
+  constexpr int P = INTER ? kRun / 2 : kRun;
+  #pragma unroll
+  for (int i = 0; i < P; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+  }
+  if (!l.turns) return;
+  int axis = 0;
+  while (axis + 1 < a.axes && l.p0 >= a.ends[axis]) ++axis;
+  if (axis + 1 < a.axes && l.p0 + P > a.ends[axis]) {
+    // the lane's pairs lie on more than one axis
+    #pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 cs = angle(a, token, l.p0 + i);
+      c[i] = cs.x;
+      s[i] = cs.y;
+    }
+    return;
+  }
+  const long at = a.pos ? a.pos[axis * a.tokens + token] : in_seq;
+  if (at < 0 || at >= a.table) {
+    #pragma unroll
+    for (int i = 0; i < P; ++i) c[i] = s[i] = __uint_as_float(0x7fc00000);
+    return;
+  }
+  const float4* cr = (const float4*)(a.cosines + at * a.half + l.p0);
+  const float4* sr = (const float4*)(a.sines + at * a.half + l.p0);
+  #pragma unroll
+  for (int i = 0; i < P / 4; ++i) {
+    const float4 cv = cr[i], sv = sr[i];
+    c[4 * i] = cv.x, c[4 * i + 1] = cv.y;
+    c[4 * i + 2] = cv.z, c[4 * i + 3] = cv.w;
+    s[4 * i] = sv.x, s[4 * i + 1] = sv.y;
+    s[4 * i + 2] = sv.z, s[4 * i + 3] = sv.w;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void weights(const Args& a, const Side& s, int e0,
+                                        bool on, float (&w)[kRun]) {
+  #pragma unroll
+  for (int e = 0; e < kRun; ++e) w[e] = on ? 1.f : 0.f;
+  if (!on || !s.w) return;
+  if (a.w_fp32) unpack<float>(*(const Run<float>*)((const float*)s.w + e0), w);
+  else unpack<T>(*(const Run<T>*)((const T*)s.w + e0), w);
+}
+
+// Work of a wave: the heads [h0, h1) of a token, queries before keys.
+struct Item {
+  long token, seq_no, in_seq;
+  int h0, h1;
+};
+
+__device__ __forceinline__ Item item_of(const Args& a, long item, int chunks,
+                                        int per) {
+  Item it;
+  it.token = item / chunks;
+  it.h0 = (int)(item % chunks) * per;
+  it.h1 = min(it.h0 + per, a.side[0].heads + a.side[1].heads);
+  it.seq_no = it.token / a.seq;
+  it.in_seq = it.token % a.seq;
+  return it;
+}
+
+template <typename T, int G, bool INTER>
+__device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
+                                         const Lane& l, const Item& it,
+                                         int h0, int h1,
+                                         const float (&w)[kRun],
+                                         const float (&wo)[kRun],
+                                         const float* c, const float* sn) {
+  const int group = (threadIdx.x & 63) / G;
+  const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss + l.e0;
+  T* y = (T*)s.y + it.token * s.heads * a.dim + l.e0;
+  const float inv_dim = 1.f / (float)a.dim;
+  for (int h = h0 + group; h < h1; h += 64 / G) {
+    Run<T> raw = (Run<T>)(T)0.f;
+    if (l.on) raw = *(const Run<T>*)(x + h * s.sh);
+    float v[kRun], o[kRun];
+    unpack(raw, v);
+    float sum = 0.f;
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) sum += v[e] * v[e];
+    const float r =
+        __builtin_amdgcn_rsqf(row_sum<G>(sum) * inv_dim + a.eps);
+    if (INTER) {
+      #pragma unroll
+      for (int i = 0; i < kRun / 2; ++i) {
+        const float p = v[2 * i] * r * w[2 * i];
+        const float q = v[2 * i + 1] * r * w[2 * i + 1];
+        o[2 * i] = p * c[i] - q * sn[i];
+        o[2 * i + 1] = q * c[i] + p * sn[i];
+      }
+    } else {
+      float vo[kRun];
+      unpack(from_lane<T>(raw, l.other), vo);
+      #pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        o[e] = v[e] * r * w[e] * c[e] +
+               l.sign * sn[e] * (vo[e] * r * wo[e]);
+    }
+    if (l.on) {
+      Run<T> out;
+      #pragma unroll
+      for (int e = 0; e < kRun; ++e) out[e] = (T)o[e];
+      *(Run<T>*)(y + (long)h * a.dim) = out;
+    }
+  }
+}
+
+template <typename T, int G, bool INTER>
+__global__ __launch_bounds__(kThreads) void fwd_rows_kernel(Args a,
+                                                            int chunks,
+                                                            int per) {
+  constexpr int P = INTER ? kRun / 2 : kRun;
+  const Lane l = lane_of<G, INTER>(a);
+  const int hq = a.side[0].heads;
+  float wq[kRun], wk[kRun], woq[kRun], wok[kRun];
+  weights<T>(a, a.side[0], l.e0, l.on, wq);
+  weights<T>(a, a.side[1], l.e0, l.on, wk);
+  if (!INTER) {
+    const int eo = (l.other % G) * kRun;
+    weights<T>(a, a.side[0], eo, l.on, woq);
+    weights<T>(a, a.side[1], eo, l.on, wok);
+  }
+  const long items = a.tokens * chunks;
+  for (long i = (long)blockIdx.x * kWaves + (threadIdx.x >> 6); i < items;
+       i += (long)gridDim.x * kWaves) {
+    const Item it = item_of(a, i, chunks, per);
+    float c[P], sn[P];
+    angles<INTER>(a, l, it.token, it.in_seq, c, sn);
+    fwd_side<T, G, INTER>(a, a.side[0], l, it, it.h0, min(it.h1, hq), wq,
+                          woq, c, sn);
+    fwd_side<T, G, INTER>(a, a.side[1], l, it, max(it.h0 - hq, 0),
+                          it.h1 - hq, wk, wok, c, sn);
+  }
+}
+
+template <typename T, int G, bool INTER>
+__device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
+                                         const Lane& l, const Item& it,
+                                         int h0, int h1,
+                                         const float (&w)[kRun],
+                                         float (&dw)[kRun], const float* c,
+                                         const float* sn) {
+  const int group = (threadIdx.x & 63) / G;
+  const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss + l.e0;
+  const long row0 = it.token * s.heads * a.dim + l.e0;
+  const T* dy = (const T*)s.dy + row0;
+  T* dx = (T*)s.y + row0;
+  const float inv_dim = 1.f / (float)a.dim;
+  for (int h = h0 + group; h < h1; h += 64 / G) {
+    Run<T> raw = (Run<T>)(T)0.f, rawd = raw;
+    if (l.on) {
+      raw = *(const Run<T>*)(x + h * s.sh);
+      rawd = *(const Run<T>*)(dy + (long)h * a.dim);
+    }
+    float v[kRun], d[kRun], dn[kRun];
+    unpack(raw, v);
+    unpack(rawd, d);
+    if (INTER) {
+      #pragma unroll
+      for (int i = 0; i < kRun / 2; ++i) {
+        dn[2 * i] = d[2 * i] * c[i] + d[2 * i + 1] * sn[i];
+        dn[2 * i + 1] = d[2 * i + 1] * c[i] - d[2 * i] * sn[i];
+      }
+    } else {
+      float dp[kRun];
+      unpack(from_lane<T>(rawd, l.other), dp);
+      #pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        dn[e] = d[e] * c[e] - l.sign * sn[e] * dp[e];
+    }
+    float sum = 0.f, dot = 0.f;
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      sum += v[e] * v[e];
+      dot += dn[e] * w[e] * v[e];
+    }
+    const float r =
+        __builtin_amdgcn_rsqf(row_sum<G>(sum) * inv_dim + a.eps);
+    const float k = row_sum<G>(dot) * inv_dim * r * r;
+    Run<T> out;
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      out[e] = (T)(r * (dn[e] * w[e] - v[e] * k));
+      dw[e] += dn[e] * v[e] * r;
+    }
+    if (l.on) *(Run<T>*)(dx + (long)h * a.dim) = out;
+  }
+}
+
+// partial[block]: dw of the queries, then of the keys.
+template <typename T, int G, bool INTER>
+__global__ __launch_bounds__(kThreads) void bwd_rows_kernel(
+    Args a, int chunks, int per, float* __restrict__ partial) {
+  constexpr int P = INTER ? kRun / 2 : kRun;
+  const Lane l = lane_of<G, INTER>(a);
+  const int hq = a.side[0].heads, wave = threadIdx.x >> 6;
+  float w[2][kRun], dw[2][kRun];
+  #pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    weights<T>(a, a.side[side], l.e0, l.on, w[side]);
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) dw[side][e] = 0.f;
+  }
+  const long items = a.tokens * chunks;
+  for (long i = (long)blockIdx.x * kWaves + wave; i < items;
+       i += (long)gridDim.x * kWaves) {
+    const Item it = item_of(a, i, chunks, per);
+    float c[P], sn[P];
+    angles<INTER>(a, l, it.token, it.in_seq, c, sn);
+    bwd_side<T, G, INTER>(a, a.side[0], l, it, it.h0, min(it.h1, hq), w[0],
+                          dw[0], c, sn);
+    bwd_side<T, G, INTER>(a, a.side[1], l, it, max(it.h0 - hq, 0),
+                          it.h1 - hq, w[1], dw[1], c, sn);
+  }
+  if (!partial) return;
+  // over the wave's groups, then over the block's waves
+  __shared__ float sums[kWaves][2][G * kRun];
+  #pragma unroll
+  for (int side = 0; side < 2; ++side)
+    #pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      float v = dw[side][e];
+      #pragma unroll
+      for (int off = G; off < 64; off *= 2) v += __shfl_xor(v, off);
+      if ((threadIdx.x & 63) < G) sums[wave][side][l.e0 + e] = v;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) {
+    const int side = i >= a.dim, e = side ? i - a.dim : i;
+    float v = 0.f;
+    #pragma unroll
+    for (int wv = 0; wv < kWaves; ++wv) v += sums[wv][side][e];
+    partial[(long)blockIdx.x * 2 * a.dim + i] = v;
+  }
+}
+
+// dw of both sides from the blocks' sums, added in a fixed order: a block
+// for 8 columns, 32 threads a column.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dw_rows_kernel(
+    const float* __restrict__ partial, void* dwq, void* dwk, int blocks,
+    int dim, bool fp32) {
+  __shared__ double sums[kThreads];
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7);
+  double v = 0.;
+  if (col < 2 * dim) {
+    #pragma unroll 8
+    for (int b = threadIdx.x >> 3; b < blocks; b += kThreads / 8)
+      v += (double)partial[(long)b * 2 * dim + col];
+  }
+  sums[threadIdx.x] = v;
+  for (int half = kThreads / 2; half >= 8; half /= 2) {
+    __syncthreads();
+    if ((int)threadIdx.x < half)
+      sums[threadIdx.x] += sums[threadIdx.x + half];
+  }
+  if (threadIdx.x >= 8 || col >= 2 * dim) return;
+  const int e = col < dim ? col : col - dim;
+  void* out = col < dim ? dwq : dwk;
+  if (!out) return;
+  const float sum = (float)sums[threadIdx.x];
+  if (fp32) ((float*)out)[e] = sum;
+  else ((T*)out)[e] = (T)sum;
+}
+
 // dw of one side from the blocks' sums, added in their order.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void dw_kernel(
@@ -316,6 +665,46 @@ void share(const Args& a, long most, int& q_blocks, int& blocks) {
   blocks = q_blocks + (int)part(rk);
 }
 
+// Whether the kernels with rows in registers take the call.
+bool fits(const Args& a, size_t elem) {
+  if (a.dim % kRun || a.dim > 64 * kRun) return false;
+  if (a.half % (a.interleaved ? kRun / 2 : kRun)) return false;
+  if (!elem::aligned16(a.cosines) || !elem::aligned16(a.sines)) return false;
+  for (const Side& s : a.side) {
+    if (!elem::aligned16(s.x) || !elem::aligned16(s.dy) ||
+        !elem::aligned16(s.w))
+      return false;
+    const long step = 16 / (long)elem;
+    if (s.sb % step || s.ss % step || s.sh % step) return false;
+  }
+  return true;
+}
+
+// Heads of a wave: all of a token's where the tokens alone fill the chip,
+// else so few that the waves do.
+void divide(const Args& a, int lanes, int& chunks, int& per) {
+  const int at_once = 64 / lanes;
+  const long heads = a.side[0].heads + a.side[1].heads;
+  const long most = (heads + at_once - 1) / at_once;
+  const long want = (8192 + a.tokens - 1) / a.tokens;
+  const long n = std::min(want, most);
+  per = (int)((most + n - 1) / n * at_once);
+  chunks = (int)((heads + per - 1) / per);
+}
+
+// Calls f with the lanes of a row and the pair layout as constants.
+template <typename F>
+void with_layout(const Args& a, F f) {
+  auto inter = [&](auto lanes) {
+    if (a.interleaved) f(lanes, std::true_type{});
+    else f(lanes, std::false_type{});
+  };
+  if (a.dim <= 8 * kRun) inter(std::integral_constant<int, 8>{});
+  else if (a.dim <= 16 * kRun) inter(std::integral_constant<int, 16>{});
+  else if (a.dim <= 32 * kRun) inter(std::integral_constant<int, 32>{});
+  else inter(std::integral_constant<int, 64>{});
+}
+
 }  // namespace
 
 std::vector<at::Tensor> qk_norm_rope_fwd(
@@ -328,13 +717,24 @@ std::vector<at::Tensor> qk_norm_rope_fwd(
   auto yk = at::empty(k.sizes(), k.options());
   const Args a = make_args(q, k, wq, wk, cosines, sines, pos, sections, eps,
                            interleaved, yq, yk);
-  int q_blocks, blocks;
-  share(a, 65536, q_blocks, blocks);
+  if (a.tokens * (a.side[0].heads + a.side[1].heads) == 0) return {yq, yk};
   STOKE_ELEM_SWITCH(q.scalar_type(), "qk_norm_rope", {
-    if (blocks > 0)
+    if (fits(a, sizeof(T))) {
+      with_layout(a, [&](auto lanes, auto inter) {
+        int chunks, per;
+        divide(a, lanes, chunks, per);
+        const long blocks = (a.tokens * chunks + kWaves - 1) / kWaves;
+        hipLaunchKernelGGL((fwd_rows_kernel<T, lanes, inter>),
+                           dim3((unsigned)std::min(blocks, 1L << 20)),
+                           dim3(kThreads), 0, elem::stream(), a, chunks, per);
+      });
+    } else {
+      int q_blocks, blocks;
+      share(a, 65536, q_blocks, blocks);
       hipLaunchKernelGGL((fwd_any_kernel<T>), dim3((unsigned)blocks),
                          dim3(kThreads), kWaves * a.dim * sizeof(float),
                          elem::stream(), a, q_blocks);
+    }
   });
   return {yq, yk};
 }
@@ -357,25 +757,51 @@ std::vector<at::Tensor> qk_norm_rope_bwd(
               "qk_norm_rope: contiguous gradients of the outputs' shape");
   a.side[0].dy = dyq.data_ptr();
   a.side[1].dy = dyk.data_ptr();
-  int q_blocks, blocks;
-  share(a, 2048, q_blocks, blocks);
-  auto partial = at::empty({blocks, a.dim}, q.options().dtype(at::kFloat));
   at::Tensor dwq, dwk;
   if (wq) dwq = at::empty(wq->sizes(), wq->options());
   if (wk) dwk = at::empty(wk->sizes(), wk->options());
+  if (a.tokens * (a.side[0].heads + a.side[1].heads) == 0) {
+    if (wq) dwq.zero_();
+    if (wk) dwk.zero_();
+    return {dq, dk, dwq, dwk};
+  }
+  void* out_q = wq ? dwq.data_ptr() : nullptr;
+  void* out_k = wk ? dwk.data_ptr() : nullptr;
+  const auto f32 = q.options().dtype(at::kFloat);
   STOKE_ELEM_SWITCH(q.scalar_type(), "qk_norm_rope", {
-    if (blocks > 0)
+    if (fits(a, sizeof(T))) {
+      with_layout(a, [&](auto lanes, auto inter) {
+        int chunks, per;
+        divide(a, lanes, chunks, per);
+        const long blocks =
+            std::min((a.tokens * chunks + kWaves - 1) / kWaves, 1024L);
+        at::Tensor partial;
+        if (wq || wk) partial = at::empty({blocks, 2 * a.dim}, f32);
+        hipLaunchKernelGGL((bwd_rows_kernel<T, lanes, inter>),
+                           dim3((unsigned)blocks), dim3(kThreads), 0,
+                           elem::stream(), a, chunks, per,
+                           wq || wk ? partial.data_ptr<float>() : nullptr);
+        if (wq || wk)
+          hipLaunchKernelGGL((dw_rows_kernel<T>),
+                             dim3((unsigned)(2 * a.dim + 7) / 8),
+                             dim3(kThreads), 0, elem::stream(),
+                             partial.data_ptr<float>(), out_q, out_k,
+                             (int)blocks, a.dim, a.w_fp32);
+      });
+    } else {
+      int q_blocks, blocks;
+      share(a, 2048, q_blocks, blocks);
+      auto partial = at::empty({blocks, a.dim}, f32);
       hipLaunchKernelGGL((bwd_any_kernel<T>), dim3((unsigned)blocks),
                          dim3(kThreads), 2 * kWaves * a.dim * sizeof(float),
                          elem::stream(), a, q_blocks,
                          partial.data_ptr<float>());
-    if (wq || wk)
-      hipLaunchKernelGGL((dw_kernel<T>), dim3((a.dim + 15) / 16, 2),
-                         dim3(kThreads), 0, elem::stream(),
-                         partial.data_ptr<float>(),
-                         wq ? dwq.data_ptr() : nullptr,
-                         wk ? dwk.data_ptr() : nullptr, q_blocks, blocks,
-                         a.dim, a.w_fp32);
+      if (wq || wk)
+        hipLaunchKernelGGL((dw_kernel<T>), dim3((a.dim + 15) / 16, 2),
+                           dim3(kThreads), 0, elem::stream(),
+                           partial.data_ptr<float>(), out_q, out_k, q_blocks,
+                           blocks, a.dim, a.w_fp32);
+    }
   });
   return {dq, dk, dwq, dwk};
 }

@@ -24,7 +24,6 @@ namespace {
 using elem::kVec;
 
 constexpr int kThreads = 256;
-constexpr float kNegInf = -__builtin_huge_valf();
 
 struct Shape {
   long rows, vocab;        // rows = outer * inner
@@ -43,37 +42,82 @@ __device__ __forceinline__ bool is_live(long t, long vocab, long ignore) {
   return t != ignore && t >= 0 && t < vocab;
 }
 
-// (M, sum) of two pieces of a row.  A piece without a finite maximum keeps
-// its sum as it is: exp(-inf - -inf) would be NaN where nothing was seen.
+// exp(d), d <= 0.  log2 e comes in two parts: with the rounded constant alone
+// every term would be off the same way (1.3e-8 |d|), and that does not
+// average out over the tokens of a sequence.
+__device__ __forceinline__ float exp_neg(float d) {
+  const float t = d * 1.925963033500011e-08f;
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.4426950216293335f, t));
+}
+
+// (M, sum) of two pieces of a row.
 __device__ __forceinline__ void join(float& m, float& s, float mo, float so) {
   const float top = fmaxf(m, mo);
-  const float a = m == top ? 1.f : __expf(m - top);
-  const float b = mo == top ? 1.f : __expf(mo - top);
-  s = s * a + so * b;
+  s = s * exp_neg(m - top) + so * exp_neg(mo - top);
   m = top;
 }
 
+// Elements of `row` up to the first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p) {
+  return (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) /
+         (int)sizeof(T);
+}
+
+// One value, or a few at once, into a thread's (M, sum).  M starts at the
+// lowest finite value, so -inf adds exp(-inf) = 0 and never meets -inf - -inf;
+// +inf and NaN make the sum NaN.
+template <int N>
+__device__ __forceinline__ void take(const float (&v)[N], float& m,
+                                     float& sum) {
+  float top = v[0];
+  #pragma unroll
+  for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
+  if (top > m) {
+    sum *= exp_neg(m - top);
+    m = top;
+  }
+  float add = 0.f;
+  #pragma unroll
+  for (int e = 0; e < N; ++e) add += exp_neg(v[e] - m);
+  sum += add;
+}
+
 // One block for each (row, piece of the vocabulary): stats[row, piece].
+// A row starts at any element (odd vocabularies): the few up to a 16-byte
+// boundary and behind the last whole 16 bytes are taken one by one.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void row_stats_kernel(
     const T* __restrict__ logits, const long* __restrict__ target,
     float2* __restrict__ stats, unsigned* __restrict__ ticket, Shape s,
     long ignore, int pieces, long piece) {
+  constexpr int V = kVec<T>;
+  using Vec = elem::vec<T, V>;
   const long row = blockIdx.x;
   const int part = blockIdx.y;
   if (row == 0 && part == 0 && threadIdx.x == 0 && ticket) *ticket = 0;
   if (!is_live(target[row], s.vocab, ignore)) return;
-  const T* x = row_of(logits, s, row);
-  const long end = min(s.vocab, (part + 1) * piece);
-  float m = kNegInf, sum = 0.f;
-  for (long i = part * piece + threadIdx.x; i < end; i += kThreads) {
-    const float v = (float)x[i];
-    if (v > m) {
-      sum *= __expf(m - v);
-      m = v;
-    }
-    // +inf - +inf: the row has no distribution, NaN as torch has it
-    if (v != kNegInf) sum += __expf(v - m);
+  const long begin = part * piece;
+  const T* x = row_of(logits, s, row) + begin;
+  const int n = (int)(min(s.vocab, begin + piece) - begin);
+  const int head = min(head_of(x), n);
+  const int body = (n - head) / V;
+  float m = -3.402823466e38f, sum = 0.f;
+  const Vec* xv = (const Vec*)(x + head);
+  #pragma unroll 4
+  for (int i = threadIdx.x; i < body; i += kThreads) {
+    const Vec w = xv[i];
+    float v[V];
+    #pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (float)w[e];
+    take(v, m, sum);
+  }
+  const int rest = n - body * V;  // head and tail
+  if ((int)threadIdx.x < rest) {
+    const int i = (int)threadIdx.x < head ? (int)threadIdx.x
+                                          : (int)threadIdx.x + body * V;
+    const float v[1] = {(float)x[i]};
+    take(v, m, sum);
   }
   #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
@@ -293,10 +337,12 @@ __global__ __launch_bounds__(kThreads) void lp_bwd_kernel(
     const float4* __restrict__ saved, const float* __restrict__ up,
     int up_step, const float* __restrict__ scale, T* __restrict__ dlogits,
     Shape s, long ignore, long piece) {
+  constexpr int V = kVec<T>;
+  using Vec = elem::vec<T, V>;
   const long row = blockIdx.x;
   const long begin = blockIdx.y * piece;
-  const long end = min(s.vocab, begin + piece);
-  T* dx = dlogits + row * s.vocab;
+  const int n = (int)(min(s.vocab, begin + piece) - begin);
+  T* dx = dlogits + row * s.vocab + begin;
   const long t = target[row];
   const float4 r = saved[row];
   float c = 0.f;
@@ -304,19 +350,42 @@ __global__ __launch_bounds__(kThreads) void lp_bwd_kernel(
     c = r.w * up[row * up_step];
     if (scale) c *= *scale;
   }
+  const int head = min(head_of(dx), n);
+  const int body = (n - head) / V;
+  const int rest = n - body * V;
+  const int lone = (int)threadIdx.x < head ? (int)threadIdx.x
+                                           : (int)threadIdx.x + body * V;
+  Vec* dv = (Vec*)(dx + head);
   if (c == 0.f) {
-    for (long i = begin + threadIdx.x; i < end; i += kThreads)
-      dx[i] = (T)0.f;
+    const Vec zero = (Vec)(T)0.f;
+    for (int i = threadIdx.x; i < body; i += kThreads) dv[i] = zero;
+    if ((int)threadIdx.x < rest) dx[lone] = (T)0.f;
     return;
   }
-  const T* x = row_of(logits, s, row);
+  const T* x = row_of(logits, s, row) + begin;
   const float k = -c * r.y;
   // 1 - p of a token that is almost certain loses its digits
-  const float at_target = -c * expm1f(r.z);
-  for (long i = begin + threadIdx.x; i < end; i += kThreads) {
-    const float p = __expf((float)x[i] - r.x);
-    dx[i] = (T)(i == t ? at_target : k * p);
+  const T at_target = (T)(-c * expm1f(r.z));
+  const long at = t - begin;  // may lie in another piece
+  if (head_of(x) == head_of(dx)) {
+    const Vec* xv = (const Vec*)(x + head);
+    #pragma unroll 4
+    for (int i = threadIdx.x; i < body; i += kThreads) {
+      const Vec w = xv[i];
+      Vec o;
+      #pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = (T)(k * exp_neg((float)w[e] - r.x));
+      dv[i] = o;
+    }
+    if ((int)threadIdx.x < rest)
+      dx[lone] = (T)(k * exp_neg((float)x[lone] - r.x));
+  } else {
+    // logits of another row stride: their 16 bytes do not match the gradient's
+    for (int i = threadIdx.x; i < n; i += kThreads)
+      dx[i] = (T)(k * exp_neg((float)x[i] - r.x));
   }
+  __syncthreads();  // the target's own value last
+  if (threadIdx.x == 0 && at >= 0 && at < n) dx[at] = at_target;
 }
 
 struct Call {
@@ -330,7 +399,9 @@ struct Call {
 void split(long rows, long vocab, int& pieces, long& piece) {
   long want = (1024 + rows - 1) / rows;
   want = std::max<long>(1, std::min<long>(want, (vocab + 4095) / 4096));
+  // whole 16 bytes, so that all pieces of a row are aligned alike
   piece = (vocab + want - 1) / want;
+  piece = (piece + 7) / 8 * 8;
   pieces = (int)((vocab + piece - 1) / piece);
 }
 
@@ -349,8 +420,9 @@ Call check(const at::Tensor& logits, const at::Tensor& target, long ignore,
               std::max<long>(1, logits.size(1)), logits.stride(0),
               logits.stride(1)};
   // a launch has fewer than 2^32 threads along x
-  TORCH_CHECK(c.s.rows < (1L << 24) && (c.s.vocab > 0 || c.s.rows == 0),
-              what, ": fewer than 2^24 rows of at least one logit required");
+  TORCH_CHECK(c.s.rows < (1L << 24) && c.s.vocab < (1L << 30) &&
+                  (c.s.vocab > 0 || c.s.rows == 0),
+              what, ": fewer than 2^24 rows of 1 to 2^30 - 1 logits required");
   c.ignore = ignore;
   if (c.s.rows > 0) split(c.s.rows, c.s.vocab, c.pieces, c.piece);
   return c;
