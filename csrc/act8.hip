@@ -285,6 +285,59 @@ struct Held {
   }
 };
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor swiglu8_forward(const at::Tensor& g, const at::Tensor& u,
+                           at::Tensor& held) {
+  const c10::DeviceGuard guard(g.device());
+  const long n = g.numel();
+  auto y = at::empty(g.sizes(), g.options());
+  held = at::empty({Held(nullptr, n).bytes}, g.options().dtype(at::kByte));
+  if (n == 0) return y;
+  const Held h(held.data_ptr(), n);
+  STOKE_ELEM_SWITCH(g.scalar_type(), "swiglu8", {
+    const long first = first_of(n, g.data_ptr(), u.data_ptr());
+    hipLaunchKernelGGL((swiglu8_fwd_kernel<T>), grid_for(n, first),
+                       dim3(kThreads), 0, elem::stream(),
+                       (const T*)g.data_ptr(), (const T*)u.data_ptr(),
+                       (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first);
+  });
+  return y;
+}
+
+variable_list swiglu8_backward(const at::Tensor& dy, const at::Tensor& held) {
+  const c10::DeviceGuard guard(dy.device());
+  const long n = dy.numel();
+  auto dg = at::empty(dy.sizes(), dy.options());
+  auto du = at::empty(dy.sizes(), dy.options());
+  if (n == 0) return {dg, du};
+  const Held h(held.data_ptr(), n);
+  STOKE_ELEM_SWITCH(dy.scalar_type(), "swiglu8", {
+    const long first = first_of(n, dy.data_ptr());
+    hipLaunchKernelGGL((swiglu8_bwd_kernel<T>), grid_for(n, first),
+                       dim3(kThreads), 0, elem::stream(),
+                       (const T*)dy.data_ptr(), h.qg, h.qu, h.sg, h.su,
+                       (T*)dg.data_ptr(), (T*)du.data_ptr(), n, first);
+  });
+  return {dg, du};
+}
+
+struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& g,
+                            const at::Tensor& u) {
+    at::Tensor held;
+    auto y = swiglu8_forward(g.contiguous(), u.contiguous(), held);
+    ctx->save_for_backward({held});
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    return elem::once_differentiable(swiglu8_backward(
+        dy[0].contiguous(), ctx->get_saved_variables()[0]));
+  }
+};
+
 }  // namespace
 
 std::vector<at::Tensor> act8_pack(at::Tensor x) {
@@ -328,47 +381,15 @@ at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype) {
   return x;
 }
 
-std::vector<at::Tensor> swiglu8_fwd(at::Tensor g, at::Tensor u) {
-  TORCH_CHECK(g.is_cuda() && u.device() == g.device() &&
-                  g.is_contiguous() && u.is_contiguous() &&
-                  g.sizes() == u.sizes() &&
-                  g.scalar_type() == u.scalar_type(),
-              "swiglu8: gate and up must be contiguous GPU tensors of one "
-              "shape and dtype");
-  const c10::DeviceGuard guard(g.device());
-  const long n = g.numel();
-  auto y = at::empty_like(g);
-  auto held = at::empty({Held(nullptr, n).bytes},
-                        g.options().dtype(at::kByte));
-  const Held h(held.data_ptr(), n);
-  STOKE_ELEM_SWITCH(g.scalar_type(), "swiglu8", {
-    const long first = first_of(n, g.data_ptr(), u.data_ptr());
-    if (n > 0)
-      hipLaunchKernelGGL((swiglu8_fwd_kernel<T>), grid_for(n, first),
-                         dim3(kThreads), 0, elem::stream(),
-                         (const T*)g.data_ptr(), (const T*)u.data_ptr(),
-                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first);
-  });
-  return {y, held};
-}
-
-std::vector<at::Tensor> swiglu8_bwd(at::Tensor dy, at::Tensor held) {
-  const long n = dy.numel();
-  const Held h(held.data_ptr(), n);
-  TORCH_CHECK(dy.is_cuda() && dy.is_contiguous() &&
-                  held.device() == dy.device() && held.numel() == h.bytes,
-              "swiglu8: gradient must be a contiguous GPU tensor of the "
-              "output's shape");
-  const c10::DeviceGuard guard(dy.device());
-  auto dg = at::empty_like(dy);
-  auto du = at::empty_like(dy);
-  STOKE_ELEM_SWITCH(dy.scalar_type(), "swiglu8", {
-    const long first = first_of(n, dy.data_ptr());
-    if (n > 0)
-      hipLaunchKernelGGL((swiglu8_bwd_kernel<T>), grid_for(n, first),
-                         dim3(kThreads), 0, elem::stream(),
-                         (const T*)dy.data_ptr(), h.qg, h.qu, h.sg, h.su,
-                         (T*)dg.data_ptr(), (T*)du.data_ptr(), n, first);
-  });
-  return {dg, du};
+// The entry point: checks its arguments, and has gradients for both.
+at::Tensor swiglu8(at::Tensor g, at::Tensor u) {
+  TORCH_CHECK_VALUE(
+      g.is_cuda() && g.sizes() == u.sizes() && g.device() == u.device() &&
+          g.scalar_type() == u.scalar_type() &&
+          (g.scalar_type() == at::kBFloat16 ||
+           g.scalar_type() == at::kHalf || g.scalar_type() == at::kFloat),
+      "Stoke -- swiglu(save_bits=8) takes gate and up of one shape, device "
+      "and dtype (bf16, fp16, fp32), got ", g.sizes(), " ", g.scalar_type(),
+      " and ", u.sizes(), " ", u.scalar_type());
+  return SwiGLU8::apply(g, u);
 }

@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 namespace elem {
 
@@ -23,6 +24,19 @@ inline hipStream_t stream() {
 
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// Gradients of a kernel without a derivative of its own: a second backward
+// through them raises instead of being taken for zero.
+inline torch::autograd::variable_list once_differentiable(
+    torch::autograd::variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "Stoke -- a fused operator was differentiated twice",
+      (int64_t)grads.size());
+  return (*node)(std::move(grads));
 }
 
 }  // namespace elem

@@ -568,88 +568,55 @@ __global__ __launch_bounds__(kThreads) void dw_kernel(
   else ((T*)out)[col] = (T)(float)v;
 }
 
-void check_side(const at::Tensor& x, const at::Tensor& like,
-                const c10::optional<at::Tensor>& w, const char* what) {
-  TORCH_CHECK(x.is_cuda() && x.device() == like.device() && x.dim() == 4 &&
-                  x.scalar_type() == like.scalar_type() &&
-                  x.size(0) == like.size(0) && x.size(1) == like.size(1) &&
-                  x.size(3) == like.size(3) &&
-                  (x.size(3) <= 1 || x.stride(3) == 1),
-              "qk_norm_rope: ", what,
-              " must be [B, S, H, D] with a unit last stride");
-  TORCH_CHECK(!w || (w->device() == x.device() && w->dim() == 1 &&
-                     w->size(0) == x.size(3) && w->is_contiguous() &&
-                     (w->scalar_type() == at::kFloat ||
-                      w->scalar_type() == x.scalar_type())),
-              "qk_norm_rope: contiguous weights [D] in fp32 or the heads' "
-              "dtype required");
-}
-
 void fill_side(Side& s, const at::Tensor& x,
-               const c10::optional<at::Tensor>& w, at::Tensor& y) {
+               const at::Tensor& w, at::Tensor& y) {
   s.x = x.data_ptr();
   s.dy = nullptr;
   s.y = y.data_ptr();
-  s.w = w ? w->data_ptr() : nullptr;
+  s.w = w.defined() ? w.data_ptr() : nullptr;
   s.sb = x.stride(0);
   s.ss = x.stride(1);
   s.sh = x.stride(2);
   s.heads = (int)x.size(2);
 }
 
-Args make_args(const at::Tensor& q, const at::Tensor& k,
-               const c10::optional<at::Tensor>& wq,
-               const c10::optional<at::Tensor>& wk, const at::Tensor& cosines,
-               const at::Tensor& sines, const c10::optional<at::Tensor>& pos,
-               const std::vector<int64_t>& sections, double eps,
-               bool interleaved, at::Tensor& yq, at::Tensor& yk) {
-  check_side(q, q, wq, "q");
-  check_side(k, q, wk, "k");
-  TORCH_CHECK(!wq || !wk || wq->scalar_type() == wk->scalar_type(),
-              "qk_norm_rope: weights of one dtype required");
+// What a call does besides its tensors.
+struct Mode {
+  std::vector<int64_t> sections;  // empty: one axis
+  double eps;
+  bool interleaved;
+};
+
+// The tensors of a call as the kernels take them: heads with a unit last
+// stride, weights, tables and positions contiguous.
+struct Tensors {
+  at::Tensor q, k, wq, wk, cosines, sines, pos;  // undefined where absent
+};
+
+Args make_args(const Tensors& t, const Mode& m, at::Tensor& yq,
+               at::Tensor& yk) {
   Args a;
-  a.tokens = q.size(0) * q.size(1);
-  a.seq = std::max<long>(1, q.size(1));
-  a.dim = (int)q.size(3);
-  TORCH_CHECK(a.dim >= 1 && a.dim <= kMaxDim,
-              "qk_norm_rope: head dim of 1 to ", kMaxDim, " required");
-  TORCH_CHECK(cosines.device() == q.device() && cosines.dim() == 2 &&
-                  cosines.scalar_type() == at::kFloat &&
-                  cosines.is_contiguous() && sines.device() == q.device() &&
-                  sines.sizes() == cosines.sizes() &&
-                  sines.scalar_type() == at::kFloat && sines.is_contiguous() &&
-                  2 * cosines.size(1) <= a.dim,
-              "qk_norm_rope: contiguous fp32 tables [P, <= D / 2] required");
-  a.table = cosines.size(0);
-  a.half = (int)cosines.size(1);
-  a.cosines = cosines.data_ptr<float>();
-  a.sines = sines.data_ptr<float>();
-  a.axes = std::max<int>(1, (int)sections.size());
-  TORCH_CHECK(a.axes <= kMaxAxes, "qk_norm_rope: at most ", kMaxAxes, " axes");
+  a.tokens = t.q.size(0) * t.q.size(1);
+  a.seq = std::max<long>(1, t.q.size(1));
+  a.dim = (int)t.q.size(3);
+  a.table = t.cosines.size(0);
+  a.half = (int)t.cosines.size(1);
+  a.cosines = t.cosines.data_ptr<float>();
+  a.sines = t.sines.data_ptr<float>();
+  a.axes = std::max<int>(1, (int)m.sections.size());
   int end = 0;
   for (int i = 0; i < kMaxAxes; ++i) {
-    if (i < (int)sections.size()) end += (int)sections[i];
+    if (i < (int)m.sections.size()) end += (int)m.sections[i];
     else end = a.half;
     a.ends[i] = end;
   }
-  a.pos = nullptr;
-  if (pos) {
-    TORCH_CHECK(pos->device() == q.device() && pos->is_contiguous() &&
-                    pos->scalar_type() == at::kLong &&
-                    pos->numel() == a.axes * a.tokens,
-                "qk_norm_rope: contiguous int64 positions [axes, B, S] "
-                "required");
-    a.pos = pos->data_ptr<long>();
-  } else {
-    TORCH_CHECK(a.axes == 1 && a.table >= a.seq,
-                "qk_norm_rope: tables shorter than the sequence");
-  }
-  a.w_fp32 = (wq && wq->scalar_type() == at::kFloat) ||
-             (wk && wk->scalar_type() == at::kFloat);
-  a.interleaved = interleaved;
-  a.eps = (float)eps;
-  fill_side(a.side[0], q, wq, yq);
-  fill_side(a.side[1], k, wk, yk);
+  a.pos = t.pos.defined() ? t.pos.data_ptr<long>() : nullptr;
+  a.w_fp32 = (t.wq.defined() && t.wq.scalar_type() == at::kFloat) ||
+             (t.wk.defined() && t.wk.scalar_type() == at::kFloat);
+  a.interleaved = m.interleaved;
+  a.eps = (float)m.eps;
+  fill_side(a.side[0], t.q, t.wq, yq);
+  fill_side(a.side[1], t.k, t.wk, yk);
   return a;
 }
 
@@ -705,20 +672,16 @@ void with_layout(const Args& a, F f) {
   else inter(std::integral_constant<int, 64>{});
 }
 
-}  // namespace
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
-std::vector<at::Tensor> qk_norm_rope_fwd(
-    at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq,
-    c10::optional<at::Tensor> wk, at::Tensor cosines, at::Tensor sines,
-    c10::optional<at::Tensor> pos, std::vector<int64_t> sections, double eps,
-    bool interleaved) {
-  const c10::DeviceGuard guard(q.device());
-  auto yq = at::empty(q.sizes(), q.options());
-  auto yk = at::empty(k.sizes(), k.options());
-  const Args a = make_args(q, k, wq, wk, cosines, sines, pos, sections, eps,
-                           interleaved, yq, yk);
+variable_list forward_of(const Tensors& t, const Mode& m) {
+  const c10::DeviceGuard guard(t.q.device());
+  auto yq = at::empty(t.q.sizes(), t.q.options());
+  auto yk = at::empty(t.k.sizes(), t.k.options());
+  const Args a = make_args(t, m, yq, yk);
   if (a.tokens * (a.side[0].heads + a.side[1].heads) == 0) return {yq, yk};
-  STOKE_ELEM_SWITCH(q.scalar_type(), "qk_norm_rope", {
+  STOKE_ELEM_SWITCH(t.q.scalar_type(), "qk_norm_rope", {
     if (fits(a, sizeof(T))) {
       with_layout(a, [&](auto lanes, auto inter) {
         int chunks, per;
@@ -739,36 +702,28 @@ std::vector<at::Tensor> qk_norm_rope_fwd(
   return {yq, yk};
 }
 
-// (dq, dk, dwq, dwk); the last two empty where there is no weight.
-std::vector<at::Tensor> qk_norm_rope_bwd(
-    at::Tensor dyq, at::Tensor dyk, at::Tensor q, at::Tensor k,
-    c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
-    at::Tensor cosines, at::Tensor sines, c10::optional<at::Tensor> pos,
-    std::vector<int64_t> sections, double eps, bool interleaved) {
-  const c10::DeviceGuard guard(q.device());
-  auto dq = at::empty(q.sizes(), q.options());
-  auto dk = at::empty(k.sizes(), k.options());
-  Args a = make_args(q, k, wq, wk, cosines, sines, pos, sections, eps,
-                     interleaved, dq, dk);
-  TORCH_CHECK(dyq.sizes() == q.sizes() && dyk.sizes() == k.sizes() &&
-                  dyq.scalar_type() == q.scalar_type() &&
-                  dyk.scalar_type() == q.scalar_type() &&
-                  dyq.is_contiguous() && dyk.is_contiguous(),
-              "qk_norm_rope: contiguous gradients of the outputs' shape");
+// (dq, dk, dwq, dwk); the last two undefined where there is no weight.
+variable_list backward_of(const Tensors& t, const Mode& m,
+                          const at::Tensor& dyq, const at::Tensor& dyk) {
+  const c10::DeviceGuard guard(t.q.device());
+  auto dq = at::empty(t.q.sizes(), t.q.options());
+  auto dk = at::empty(t.k.sizes(), t.k.options());
+  Args a = make_args(t, m, dq, dk);
   a.side[0].dy = dyq.data_ptr();
   a.side[1].dy = dyk.data_ptr();
   at::Tensor dwq, dwk;
-  if (wq) dwq = at::empty(wq->sizes(), wq->options());
-  if (wk) dwk = at::empty(wk->sizes(), wk->options());
+  if (t.wq.defined()) dwq = at::empty(t.wq.sizes(), t.wq.options());
+  if (t.wk.defined()) dwk = at::empty(t.wk.sizes(), t.wk.options());
   if (a.tokens * (a.side[0].heads + a.side[1].heads) == 0) {
-    if (wq) dwq.zero_();
-    if (wk) dwk.zero_();
+    if (dwq.defined()) dwq.zero_();
+    if (dwk.defined()) dwk.zero_();
     return {dq, dk, dwq, dwk};
   }
-  void* out_q = wq ? dwq.data_ptr() : nullptr;
-  void* out_k = wk ? dwk.data_ptr() : nullptr;
-  const auto f32 = q.options().dtype(at::kFloat);
-  STOKE_ELEM_SWITCH(q.scalar_type(), "qk_norm_rope", {
+  void* out_q = dwq.defined() ? dwq.data_ptr() : nullptr;
+  void* out_k = dwk.defined() ? dwk.data_ptr() : nullptr;
+  const bool sums = dwq.defined() || dwk.defined();
+  const auto f32 = t.q.options().dtype(at::kFloat);
+  STOKE_ELEM_SWITCH(t.q.scalar_type(), "qk_norm_rope", {
     if (fits(a, sizeof(T))) {
       with_layout(a, [&](auto lanes, auto inter) {
         int chunks, per;
@@ -776,12 +731,12 @@ std::vector<at::Tensor> qk_norm_rope_bwd(
         const long blocks =
             std::min((a.tokens * chunks + kWaves - 1) / kWaves, 1024L);
         at::Tensor partial;
-        if (wq || wk) partial = at::empty({blocks, 2 * a.dim}, f32);
+        if (sums) partial = at::empty({blocks, 2 * a.dim}, f32);
         hipLaunchKernelGGL((bwd_rows_kernel<T, lanes, inter>),
                            dim3((unsigned)blocks), dim3(kThreads), 0,
                            elem::stream(), a, chunks, per,
-                           wq || wk ? partial.data_ptr<float>() : nullptr);
-        if (wq || wk)
+                           sums ? partial.data_ptr<float>() : nullptr);
+        if (sums)
           hipLaunchKernelGGL((dw_rows_kernel<T>),
                              dim3((unsigned)(2 * a.dim + 7) / 8),
                              dim3(kThreads), 0, elem::stream(),
@@ -796,7 +751,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd(
                          dim3(kThreads), 2 * kWaves * a.dim * sizeof(float),
                          elem::stream(), a, q_blocks,
                          partial.data_ptr<float>());
-      if (wq || wk)
+      if (sums)
         hipLaunchKernelGGL((dw_kernel<T>), dim3((a.dim + 15) / 16, 2),
                            dim3(kThreads), 0, elem::stream(),
                            partial.data_ptr<float>(), out_q, out_k, q_blocks,
@@ -804,4 +759,149 @@ std::vector<at::Tensor> qk_norm_rope_bwd(
     }
   });
   return {dq, dk, dwq, dwk};
+}
+
+struct QKNormRope : torch::autograd::Function<QKNormRope> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q,
+                               const at::Tensor& k,
+                               const std::optional<at::Tensor>& wq,
+                               const std::optional<at::Tensor>& wk,
+                               const Tensors& t, const Mode& m) {
+    ctx->save_for_backward({q, k, wq.value_or(at::Tensor()),
+                            wk.value_or(at::Tensor()), t.cosines, t.sines,
+                            t.pos});
+    ctx->saved_data["sections"] = m.sections;
+    ctx->saved_data["eps"] = m.eps;
+    ctx->saved_data["interleaved"] = m.interleaved;
+    return forward_of(t, m);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto v = ctx->get_saved_variables();
+    const Tensors t{v[0], v[1], v[2], v[3], v[4], v[5], v[6]};
+    const Mode m{ctx->saved_data["sections"].toIntVector(),
+                 ctx->saved_data["eps"].toDouble(),
+                 ctx->saved_data["interleaved"].toBool()};
+    const auto d = backward_of(t, m, dy[0].contiguous(), dy[1].contiguous());
+    variable_list out(6);
+    std::copy(d.begin(), d.end(), out.begin());
+    return elem::once_differentiable(std::move(out));
+  }
+};
+
+void check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq,
+           const at::Tensor& wk, const at::Tensor& cosines,
+           const at::Tensor& sines, const std::optional<at::Tensor>& pos,
+           const std::optional<std::vector<int64_t>>& sections) {
+  TORCH_CHECK_VALUE(
+      q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) &&
+          q.size(1) == k.size(1) && q.size(3) == k.size(3) &&
+          q.scalar_type() == k.scalar_type() && q.is_cuda() &&
+          q.device() == k.device() &&
+          (q.scalar_type() == at::kBFloat16 ||
+           q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat) &&
+          q.size(3) >= 1 && q.size(3) <= kMaxDim,
+      "Stoke -- qk_norm_rope takes q [B, S, H, D] and k [B, S, Hk, D] of one "
+      "floating dtype and device, D up to ", kMaxDim, ", got ", q.sizes(),
+      " ", q.scalar_type(), " and ", k.sizes(), " ", k.scalar_type());
+  for (const at::Tensor& w : {wq, wk})
+    TORCH_CHECK_VALUE(
+        !w.defined() ||
+            (w.dim() == 1 && w.size(0) == q.size(3) &&
+             w.device() == q.device() &&
+             (w.scalar_type() == at::kFloat ||
+              w.scalar_type() == q.scalar_type())),
+        "Stoke -- qk_norm_rope weights are [", q.size(3), "] in fp32 or ",
+        q.scalar_type());
+  TORCH_CHECK_VALUE(!wq.defined() || !wk.defined() ||
+                        wq.scalar_type() == wk.scalar_type(),
+                    "Stoke -- qk_norm_rope weights have one dtype");
+  TORCH_CHECK_VALUE(
+      cosines.dim() == 2 && cosines.sizes() == sines.sizes() &&
+          cosines.device() == q.device() && sines.device() == q.device() &&
+          cosines.is_floating_point() && sines.is_floating_point() &&
+          2 * cosines.size(1) <= q.size(3) && !cosines.requires_grad() &&
+          !sines.requires_grad(),
+      "Stoke -- qk_norm_rope takes constant tables cos, sin [P, <= D / 2], "
+      "got ", cosines.sizes(), " and ", sines.sizes());
+  int64_t axes = 1;
+  if (sections) {
+    axes = (int64_t)sections->size();
+    int64_t sum = 0;
+    bool fine = axes >= 1 && axes <= kMaxAxes;
+    for (const int64_t n : *sections) {
+      fine = fine && n >= 0 && n <= cosines.size(1);
+      sum += fine ? n : 0;
+    }
+    TORCH_CHECK_VALUE(fine && sum == cosines.size(1),
+                      "Stoke -- sections are 1 to ", kMaxAxes,
+                      " numbers of pairs that add up to ", cosines.size(1),
+                      ", got ", *sections);
+  }
+  if (!pos) {
+    TORCH_CHECK_VALUE(axes == 1 && cosines.size(0) >= q.size(1),
+                      "Stoke -- without positions there is one axis and the "
+                      "tables cover the sequence (", cosines.size(0),
+                      " rows for ", q.size(1), ")");
+    return;
+  }
+  const int64_t lead = sections ? 1 : 0;
+  bool fine = (pos->scalar_type() == at::kLong ||
+               pos->scalar_type() == at::kInt) &&
+              pos->device() == q.device() && pos->dim() == lead + 2 &&
+              (!lead || pos->size(0) == axes);
+  for (int64_t i = 0; fine && i < 2; ++i)
+    fine = pos->size(lead + i) == 1 || pos->size(lead + i) == q.size(i);
+  TORCH_CHECK_VALUE(fine,
+                    "Stoke -- positions are whole numbers [axes with "
+                    "sections, B, S] (B and S of 1 broadcast) on the heads' "
+                    "device, got ", pos->sizes(), " ", pos->scalar_type());
+}
+
+at::Tensor unit_stride(const at::Tensor& x) {
+  return x.size(3) > 1 && x.stride(3) != 1 ? x.contiguous() : x;
+}
+
+at::Tensor table32(const at::Tensor& x) {
+  return x.scalar_type() == at::kFloat ? x.contiguous()
+                                       : x.to(at::kFloat).contiguous();
+}
+
+}  // namespace
+
+// The entry point: checks its arguments, and has gradients for the heads and
+// the weights.
+std::vector<at::Tensor> qk_norm_rope(
+    at::Tensor q, at::Tensor k, std::optional<at::Tensor> wq,
+    std::optional<at::Tensor> wk, at::Tensor cosines, at::Tensor sines,
+    std::optional<at::Tensor> pos,
+    std::optional<std::vector<int64_t>> sections, double eps,
+    bool interleaved) {
+  Tensors t;
+  if (wq) t.wq = wq->contiguous();
+  if (wk) t.wk = wk->contiguous();
+  check(q, k, t.wq, t.wk, cosines, sines, pos, sections);
+  t.q = unit_stride(q);
+  t.k = unit_stride(k);
+  t.cosines = table32(cosines);
+  t.sines = table32(sines);
+  if (pos) {
+    t.pos = pos->scalar_type() == at::kLong ? *pos : pos->to(at::kLong);
+    std::vector<int64_t> want = t.pos.sizes().vec();
+    want[want.size() - 2] = q.size(0);
+    want[want.size() - 1] = q.size(1);
+    if (t.pos.sizes() != at::IntArrayRef(want)) t.pos = t.pos.expand(want);
+    t.pos = t.pos.contiguous();
+  }
+  const Mode m{sections.value_or(std::vector<int64_t>()), eps, interleaved};
+  const bool grad =
+      at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() ||
+       (t.wq.defined() && t.wq.requires_grad()) ||
+       (t.wk.defined() && t.wk.requires_grad()));
+  if (!grad) return forward_of(t, m);
+  // variables among the arguments are found as tensors of their own
+  return QKNormRope::apply(
+      t.q, t.k, wq ? std::optional<at::Tensor>(t.wq) : std::nullopt,
+      wk ? std::optional<at::Tensor>(t.wk) : std::nullopt, t, m);
 }

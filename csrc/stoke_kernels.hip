@@ -693,36 +693,26 @@ std::vector<at::Tensor> fp8_quant_t(at::Tensor x, at::Tensor scale,
 // Activations held in 8 bits (csrc/act8.hip)
 std::vector<at::Tensor> act8_pack(at::Tensor x);
 at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype);
-std::vector<at::Tensor> swiglu8_fwd(at::Tensor g, at::Tensor u);
-std::vector<at::Tensor> swiglu8_bwd(at::Tensor dy, at::Tensor held);
+at::Tensor swiglu8(at::Tensor g, at::Tensor u);
 
 // Token log-probabilities and the losses on them (csrc/token_loss.hip)
-std::vector<at::Tensor> token_logprobs_fwd(at::Tensor logits,
-                                           at::Tensor target,
-                                           int64_t ignore);
-std::vector<at::Tensor> policy_loss_fwd(
-    at::Tensor logits, at::Tensor target, at::Tensor old_lp, at::Tensor adv,
-    c10::optional<at::Tensor> ref_lp, double low, double high, double kl,
-    int64_t ignore);
-std::vector<at::Tensor> preference_loss_fwd(at::Tensor logits,
-                                            at::Tensor target,
-                                            at::Tensor ref_lp, double beta,
-                                            double eps, int64_t ignore);
-at::Tensor token_loss_bwd(at::Tensor logits, at::Tensor target,
-                          at::Tensor saved, at::Tensor up,
-                          c10::optional<at::Tensor> scale, int64_t ignore);
+at::Tensor token_logprobs(at::Tensor logits, at::Tensor target,
+                          int64_t ignore);
+at::Tensor policy_loss(at::Tensor logits, at::Tensor target,
+                       at::Tensor old_lp, at::Tensor adv,
+                       std::optional<at::Tensor> ref_lp, double clip_low,
+                       double clip_high, double kl, int64_t ignore);
+std::vector<at::Tensor> preference_loss(at::Tensor logits, at::Tensor target,
+                                        at::Tensor ref_lp, double beta,
+                                        double eps, int64_t ignore);
 
 // Norm and rotation of query and key heads (csrc/qk_norm_rope.hip)
-std::vector<at::Tensor> qk_norm_rope_fwd(
-    at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq,
-    c10::optional<at::Tensor> wk, at::Tensor cosines, at::Tensor sines,
-    c10::optional<at::Tensor> pos, std::vector<int64_t> sections, double eps,
+std::vector<at::Tensor> qk_norm_rope(
+    at::Tensor q, at::Tensor k, std::optional<at::Tensor> wq,
+    std::optional<at::Tensor> wk, at::Tensor cosines, at::Tensor sines,
+    std::optional<at::Tensor> pos,
+    std::optional<std::vector<int64_t>> sections, double eps,
     bool interleaved);
-std::vector<at::Tensor> qk_norm_rope_bwd(
-    at::Tensor dyq, at::Tensor dyk, at::Tensor q, at::Tensor k,
-    c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
-    at::Tensor cosines, at::Tensor sines, c10::optional<at::Tensor> pos,
-    std::vector<int64_t> sections, double eps, bool interleaved);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &ce_fwd, "fused bf16 cross-entropy forward (online lse)");
@@ -773,20 +763,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "dynamic loss scale update (HIP)");
   m.def("act8_pack", &act8_pack, "activation to 8 bits (MXINT8)");
   m.def("act8_unpack", &act8_unpack, "activation back from 8 bits (MXINT8)");
-  m.def("swiglu8_fwd", &swiglu8_fwd,
+  m.def("swiglu8", &swiglu8,
         "silu(g)*u, keeping g and u in 8 bits for the backward");
-  m.def("swiglu8_bwd", &swiglu8_bwd, "SwiGLU backward from 8-bit inputs");
-  m.def("token_logprobs_fwd", &token_logprobs_fwd,
+  m.def("token_logprobs", &token_logprobs,
         "log-probabilities of given tokens");
-  m.def("policy_loss_fwd", &policy_loss_fwd,
-        "clipped policy loss with a KL term, forward");
-  m.def("preference_loss_fwd", &preference_loss_fwd,
-        "paired preference loss, forward");
-  m.def("token_loss_bwd", &token_loss_bwd,
-        "logits' gradient of a loss on token log-probabilities");
-  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd,
+  m.def("policy_loss", &policy_loss, "clipped policy loss with a KL term");
+  m.def("preference_loss", &preference_loss, "paired preference loss");
+  m.def("qk_norm_rope", &qk_norm_rope,
         "per-head RMS norm and rotation of queries and keys");
-  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd,
-        "gradients of the heads and weights of qk_norm_rope");
   m.attr("_built_for") = "gfx950";
 }

@@ -86,17 +86,26 @@ __device__ __forceinline__ void take(const float (&v)[N], float& m,
 // One block for each (row, piece of the vocabulary): stats[row, piece].
 // A row starts at any element (odd vocabularies): the few up to a 16-byte
 // boundary and behind the last whole 16 bytes are taken one by one.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void row_stats_kernel(
+// With FINISH (one piece a row) a row's lp is written here.
+template <typename T, int THREADS, bool FINISH>
+__global__ __launch_bounds__(THREADS) void row_stats_kernel(
     const T* __restrict__ logits, const long* __restrict__ target,
     float2* __restrict__ stats, unsigned* __restrict__ ticket, Shape s,
-    long ignore, int pieces, long piece) {
+    long ignore, int pieces, long piece, float4* __restrict__ saved,
+    float* __restrict__ lp) {
   constexpr int V = kVec<T>;
   using Vec = elem::vec<T, V>;
   const long row = blockIdx.x;
   const int part = blockIdx.y;
   if (row == 0 && part == 0 && threadIdx.x == 0 && ticket) *ticket = 0;
-  if (!is_live(target[row], s.vocab, ignore)) return;
+  const long t = target[row];
+  if (!is_live(t, s.vocab, ignore)) {
+    if (FINISH && threadIdx.x == 0) {
+      lp[row] = 0.f;
+      if (saved) saved[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
   const long begin = part * piece;
   const T* x = row_of(logits, s, row) + begin;
   const int n = (int)(min(s.vocab, begin + piece) - begin);
@@ -105,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(
   float m = -3.402823466e38f, sum = 0.f;
   const Vec* xv = (const Vec*)(x + head);
   #pragma unroll 4
-  for (int i = threadIdx.x; i < body; i += kThreads) {
+  for (int i = threadIdx.x; i < body; i += THREADS) {
     const Vec w = xv[i];
     float v[V];
     #pragma unroll
@@ -122,15 +131,21 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(
   #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
     join(m, sum, __shfl_xor(m, off), __shfl_xor(sum, off));
-  __shared__ float2 part_stats[kThreads / 64];
+  __shared__ float2 part_stats[THREADS / 64];
   if ((threadIdx.x & 63) == 0)
     part_stats[threadIdx.x >> 6] = make_float2(m, sum);
   __syncthreads();
   if (threadIdx.x == 0) {
     #pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w)
+    for (int w = 1; w < THREADS / 64; ++w)
       join(m, sum, part_stats[w].x, part_stats[w].y);
-    stats[row * pieces + part] = make_float2(m, sum);
+    if (!FINISH) {
+      stats[row * pieces + part] = make_float2(m, sum);
+      return;
+    }
+    const double l = (double)(float)x[t] - (double)m - log((double)sum);
+    lp[row] = (float)l;
+    if (saved) saved[row] = make_float4(m, 1.f / sum, (float)l, 1.f);
   }
 }
 
@@ -174,12 +189,12 @@ __global__ __launch_bounds__(kThreads) void lp_finish_kernel(
   const long t = target[row];
   if (!is_live(t, s.vocab, ignore)) {
     lp[row] = 0.f;
-    saved[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (saved) saved[row] = make_float4(0.f, 0.f, 0.f, 0.f);
     return;
   }
   const RowLp r = row_lp(logits, stats, s, row, t, pieces);
   lp[row] = (float)r.lp;
-  saved[row] = make_float4(r.m, r.inv, (float)r.lp, 1.f);
+  if (saved) saved[row] = make_float4(r.m, r.inv, (float)r.lp, 1.f);
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -388,6 +403,7 @@ __global__ __launch_bounds__(kThreads) void lp_bwd_kernel(
   if (threadIdx.x == 0 && at >= 0 && at < n) dx[at] = at_target;
 }
 
+// How a call reads the logits.
 struct Call {
   Shape s;
   long ignore;
@@ -405,167 +421,338 @@ void split(long rows, long vocab, int& pieces, long& piece) {
   pieces = (int)((vocab + piece - 1) / piece);
 }
 
-Call check(const at::Tensor& logits, const at::Tensor& target, long ignore,
-           const char* what) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3 &&
-                  (logits.size(2) <= 1 || logits.stride(2) == 1),
-              what, ": logits [B, S, V] with a unit last stride required");
-  TORCH_CHECK(target.device() == logits.device() &&
-                  target.scalar_type() == at::kLong && target.dim() == 2 &&
-                  target.size(0) == logits.size(0) &&
-                  target.size(1) == logits.size(1) && target.is_contiguous(),
-              what, ": contiguous int64 targets [B, S] required");
+// logits [rows, V] or [outer, inner, V] with a unit last stride.
+Call plan(const at::Tensor& logits, long ignore) {
+  const bool flat = logits.dim() == 2;
   Call c;
-  c.s = Shape{logits.size(0) * logits.size(1), logits.size(2),
-              std::max<long>(1, logits.size(1)), logits.stride(0),
-              logits.stride(1)};
+  c.s.vocab = logits.size(-1);
+  c.s.inner = std::max<long>(1, logits.size(-2));
+  c.s.rows = flat ? logits.size(0) : logits.size(0) * logits.size(1);
+  c.s.row_stride = logits.stride(-2);
+  c.s.outer_stride = flat ? 0 : logits.stride(0);
   // a launch has fewer than 2^32 threads along x
-  TORCH_CHECK(c.s.rows < (1L << 24) && c.s.vocab < (1L << 30) &&
-                  (c.s.vocab > 0 || c.s.rows == 0),
-              what, ": fewer than 2^24 rows of 1 to 2^30 - 1 logits required");
+  TORCH_CHECK_VALUE(c.s.rows < (1L << 22) && c.s.vocab < (1L << 30),
+                    "Stoke -- losses on logits take fewer than 2^22 "
+                    "positions of fewer than 2^30 logits");
   c.ignore = ignore;
+  c.pieces = 1;
+  c.piece = c.s.vocab;
   if (c.s.rows > 0) split(c.s.rows, c.s.vocab, c.pieces, c.piece);
   return c;
 }
 
-void check_rows(const at::Tensor& v, const at::Tensor& target,
-                const char* what) {
-  TORCH_CHECK(v.device() == target.device() && v.is_contiguous() &&
-                  v.scalar_type() == at::kFloat &&
-                  v.sizes() == target.sizes(),
-              what, ": contiguous fp32 values of the targets' shape required");
+void check(const at::Tensor& logits, const at::Tensor& target,
+           const char* what) {
+  TORCH_CHECK_VALUE(
+      logits.is_cuda() && logits.dim() >= 2 && logits.size(-1) >= 1 &&
+          (logits.scalar_type() == at::kBFloat16 ||
+           logits.scalar_type() == at::kHalf ||
+           logits.scalar_type() == at::kFloat),
+      "Stoke -- ", what, " takes floating logits [..., V], got ",
+      logits.scalar_type(), " ", logits.sizes());
+  TORCH_CHECK_VALUE(
+      target.scalar_type() == at::kLong &&
+          target.device() == logits.device() &&
+          target.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+      "Stoke -- ", what, " takes int64 targets of the logits' shape without "
+      "the vocabulary on their device, got ", target.scalar_type(), " ",
+      target.sizes(), " for logits ", logits.sizes());
 }
 
+// The kernels' layout: 2-D logits, or 3-D with any two leading strides.
+at::Tensor rows_of(const at::Tensor& logits) {
+  at::Tensor x = logits;
+  if (x.dim() > 3) x = x.flatten(0, -3);
+  if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
+  return x;
+}
+
+// Constant values for each token in contiguous fp32.
+at::Tensor per_token(const at::Tensor& v, const at::Tensor& target,
+                     const char* what) {
+  TORCH_CHECK_VALUE(!v.requires_grad(), "Stoke -- ", what,
+                    " is a constant of the loss; detach() it");
+  bool fits = v.is_floating_point() && v.device() == target.device() &&
+              v.dim() == target.dim();
+  for (int64_t i = 0; fits && i < v.dim(); ++i)
+    fits = v.size(i) == target.size(i) || v.size(i) == 1;
+  TORCH_CHECK_VALUE(fits, "Stoke -- ", what,
+                    " must hold floating values for targets ",
+                    target.sizes(), " (sizes of 1 broadcast) on their "
+                    "device, got ", v.scalar_type(), " ", v.sizes());
+  at::Tensor x = v;
+  if (x.scalar_type() != at::kFloat) x = x.to(at::kFloat);
+  if (x.sizes() != target.sizes()) x = x.expand(target.sizes());
+  return x.contiguous();
+}
+
+bool wants_grad(const at::Tensor& x) {
+  return at::GradMode::is_enabled() && x.requires_grad();
+}
+
+// Temporary memory of a forward call: the blocks' partial sums in fp64, the
+// ticket of the last block and the row statistics, in one allocation.
+struct Scratch {
+  at::Tensor store;
+  double* partial;
+  unsigned* ticket;
+  float2* stats;
+  Scratch(const at::Tensor& like, long partials, const Call& c) {
+    store = at::empty({(partials + 1 + c.s.rows * c.pieces) * 8},
+                      like.options().dtype(at::kByte));
+    partial = (double*)store.data_ptr();
+    ticket = (unsigned*)(partial + partials);
+    stats = (float2*)(partial + partials + 1);
+  }
+};
+
 template <typename T>
-at::Tensor launch_stats(const at::Tensor& logits, const at::Tensor& target,
-                        const Call& c, unsigned* ticket) {
-  auto stats = at::empty({c.s.rows, c.pieces, 2},
-                         logits.options().dtype(at::kFloat));
-  hipLaunchKernelGGL((row_stats_kernel<T>),
+void launch_stats(const at::Tensor& logits, const at::Tensor& target,
+                  const Call& c, const Scratch& tmp) {
+  hipLaunchKernelGGL((row_stats_kernel<T, kThreads, false>),
                      dim3((unsigned)c.s.rows, (unsigned)c.pieces),
                      dim3(kThreads), 0, elem::stream(),
                      (const T*)logits.data_ptr(), target.data_ptr<long>(),
-                     (float2*)stats.data_ptr(), ticket, c.s, c.ignore,
-                     c.pieces, c.piece);
-  return stats;
+                     tmp.stats, tmp.ticket, c.s, c.ignore, c.pieces, c.piece,
+                     nullptr, nullptr);
 }
 
-}  // namespace
-
-// (lp [B, S] fp32, saved [B, S, 4] fp32)
-std::vector<at::Tensor> token_logprobs_fwd(at::Tensor logits,
-                                           at::Tensor target,
-                                           int64_t ignore) {
-  const Call c = check(logits, target, ignore, "token_logprobs");
+// dlogits of a loss with `saved` row statistics.  up: one value for each row
+// (token_logprobs) or one for all (the losses).
+at::Tensor backward_of(const at::Tensor& logits, const at::Tensor& target,
+                       const float4* saved, const at::Tensor& grad,
+                       const float* scale, long ignore) {
   const c10::DeviceGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
-  auto lp = at::empty(target.sizes(), f32);
-  auto saved = at::empty({target.size(0), target.size(1), 4}, f32);
+  const Call c = plan(logits, ignore);
+  auto dlogits = at::empty(logits.sizes(), logits.options());
+  const auto up = grad.to(at::kFloat).contiguous();
+  STOKE_ELEM_SWITCH(logits.scalar_type(), "token_loss", {
+    if (c.s.rows > 0)
+      hipLaunchKernelGGL(
+          (lp_bwd_kernel<T>), dim3((unsigned)c.s.rows, (unsigned)c.pieces),
+          dim3(kThreads), 0, elem::stream(), (const T*)logits.data_ptr(),
+          target.data_ptr<long>(), saved, up.data_ptr<float>(),
+          up.numel() == 1 ? 0 : 1, scale, (T*)dlogits.data_ptr(), c.s,
+          ignore, c.piece);
+  });
+  return dlogits;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor saved_for(const at::Tensor& logits, long rows) {
+  return at::empty({4 * rows + 4}, logits.options().dtype(at::kFloat));
+}
+
+// (lp [...] fp32); saved may be undefined.
+at::Tensor logprobs_forward(const at::Tensor& logits,
+                            const at::Tensor& target, long ignore,
+                            const at::Tensor& saved) {
+  const c10::DeviceGuard guard(logits.device());
+  const Call c = plan(logits, ignore);
+  auto lp = at::empty(target.sizes(), logits.options().dtype(at::kFloat));
+  if (c.s.rows == 0) return lp;
+  float4* keep = saved.defined() ? (float4*)saved.data_ptr() : nullptr;
   STOKE_ELEM_SWITCH(logits.scalar_type(), "token_logprobs", {
-    if (c.s.rows > 0) {
-      auto stats = launch_stats<T>(logits, target, c, nullptr);
+    if (c.pieces == 1) {
+      hipLaunchKernelGGL((row_stats_kernel<T, kThreads, true>),
+                         dim3((unsigned)c.s.rows), dim3(kThreads), 0,
+                         elem::stream(), (const T*)logits.data_ptr(),
+                         target.data_ptr<long>(), nullptr, nullptr, c.s,
+                         ignore, 1, c.piece, keep, lp.data_ptr<float>());
+    } else {
+      const Scratch tmp(logits, 0, c);
+      launch_stats<T>(logits, target, c, tmp);
       hipLaunchKernelGGL(
           (lp_finish_kernel<T>),
           dim3((unsigned)((c.s.rows + kThreads - 1) / kThreads)),
           dim3(kThreads), 0, elem::stream(), (const T*)logits.data_ptr(),
-          target.data_ptr<long>(), (const float2*)stats.data_ptr(),
-          (float4*)saved.data_ptr(), lp.data_ptr<float>(), c.s, ignore,
-          c.pieces);
+          target.data_ptr<long>(), tmp.stats, keep, lp.data_ptr<float>(),
+          c.s, ignore, c.pieces);
     }
   });
-  return {lp, saved};
+  return lp;
 }
 
-// (loss [], saved [B, S, 4], inv_count [])
-std::vector<at::Tensor> policy_loss_fwd(
-    at::Tensor logits, at::Tensor target, at::Tensor old_lp, at::Tensor adv,
-    c10::optional<at::Tensor> ref_lp, double low, double high, double kl,
-    int64_t ignore) {
-  const Call c = check(logits, target, ignore, "policy_loss");
-  check_rows(old_lp, target, "policy_loss");
-  check_rows(adv, target, "policy_loss");
-  if (ref_lp) check_rows(*ref_lp, target, "policy_loss");
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits,
+                            const at::Tensor& target, int64_t ignore) {
+    auto saved = saved_for(logits, target.numel());
+    auto lp = logprobs_forward(logits, target, ignore, saved);
+    ctx->save_for_backward({logits, target, saved});
+    ctx->saved_data["ignore"] = ignore;
+    return lp;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    const auto v = ctx->get_saved_variables();
+    auto d = backward_of(v[0], v[1], (const float4*)v[2].data_ptr(), up[0],
+                         nullptr, ctx->saved_data["ignore"].toInt());
+    return elem::once_differentiable({d, at::Tensor(), at::Tensor()});
+  }
+};
+
+// saved: 4 values for each row, then 1 / (number of tokens).
+at::Tensor policy_forward(const at::Tensor& logits, const at::Tensor& target,
+                          const at::Tensor& old_lp, const at::Tensor& adv,
+                          const at::Tensor& ref_lp, const PolicyArgs& a,
+                          long ignore, at::Tensor& saved) {
   const c10::DeviceGuard guard(logits.device());
+  const Call c = plan(logits, ignore);
   const auto f32 = logits.options().dtype(at::kFloat);
-  auto saved = at::empty({target.size(0), target.size(1), 4}, f32);
-  if (c.s.rows == 0)
-    return {at::zeros({}, f32), saved, at::ones({}, f32)};
-  auto loss = at::empty({}, f32), inv_count = at::empty({}, f32);
+  saved = saved_for(logits, c.s.rows);
+  if (c.s.rows == 0) return at::zeros({}, f32);
+  auto loss = at::empty({}, f32);
   const long blocks = (c.s.rows + kThreads - 1) / kThreads;
-  auto partial = at::empty({2 * blocks + 1}, f32.dtype(at::kDouble));
-  double* part = partial.data_ptr<double>();
-  unsigned* ticket = (unsigned*)(part + 2 * blocks);
+  const Scratch tmp(logits, 2 * blocks, c);
   STOKE_ELEM_SWITCH(logits.scalar_type(), "policy_loss", {
-    auto stats = launch_stats<T>(logits, target, c, ticket);
+    launch_stats<T>(logits, target, c, tmp);
     hipLaunchKernelGGL(
         (policy_finish_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0,
         elem::stream(), (const T*)logits.data_ptr(),
-        target.data_ptr<long>(), (const float2*)stats.data_ptr(),
-        old_lp.data_ptr<float>(), adv.data_ptr<float>(),
-        ref_lp ? ref_lp->data_ptr<float>() : nullptr,
-        (float4*)saved.data_ptr(), part, ticket, loss.data_ptr<float>(),
-        inv_count.data_ptr<float>(), c.s, ignore, c.pieces,
-        PolicyArgs{low, high, kl});
+        target.data_ptr<long>(), tmp.stats, old_lp.data_ptr<float>(),
+        adv.data_ptr<float>(),
+        ref_lp.defined() ? ref_lp.data_ptr<float>() : nullptr,
+        (float4*)saved.data_ptr(), tmp.partial, tmp.ticket,
+        loss.data_ptr<float>(), saved.data_ptr<float>() + 4 * c.s.rows, c.s,
+        ignore, c.pieces, a);
   });
-  return {loss, saved, inv_count};
+  return loss;
 }
 
-// (loss [], rewards [B], saved [B, S, 4])
-std::vector<at::Tensor> preference_loss_fwd(at::Tensor logits,
-                                            at::Tensor target,
-                                            at::Tensor ref_lp, double beta,
-                                            double eps, int64_t ignore) {
-  const Call c = check(logits, target, ignore, "preference_loss");
-  check_rows(ref_lp, target, "preference_loss");
-  const long pairs = target.size(0) / 2, seq = target.size(1);
-  TORCH_CHECK(pairs > 0 && target.size(0) % 2 == 0,
-              "preference_loss: an even number of sequences required");
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits,
+                            const at::Tensor& target,
+                            const at::Tensor& old_lp, const at::Tensor& adv,
+                            const std::optional<at::Tensor>& ref_lp,
+                            double low, double high, double kl,
+                            int64_t ignore) {
+    at::Tensor saved;
+    auto loss = policy_forward(logits, target, old_lp, adv,
+                               ref_lp.value_or(at::Tensor()),
+                               PolicyArgs{low, high, kl}, ignore, saved);
+    ctx->save_for_backward({logits, target, saved});
+    ctx->saved_data["ignore"] = ignore;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    const auto v = ctx->get_saved_variables();
+    const float* saved = v[2].data_ptr<float>();
+    auto d = backward_of(v[0], v[1], (const float4*)saved, up[0],
+                         saved + 4 * v[1].numel(),
+                         ctx->saved_data["ignore"].toInt());
+    variable_list out(9);
+    out[0] = d;
+    return elem::once_differentiable(std::move(out));
+  }
+};
+
+variable_list preference_forward(const at::Tensor& logits,
+                                 const at::Tensor& target,
+                                 const at::Tensor& ref_lp, double beta,
+                                 double eps, long ignore, at::Tensor& saved) {
   const c10::DeviceGuard guard(logits.device());
+  const Call c = plan(logits, ignore);
   const auto f32 = logits.options().dtype(at::kFloat);
-  auto saved = at::empty({target.size(0), seq, 4}, f32);
+  const long pairs = target.size(0) / 2, seq = target.size(1);
+  saved = saved_for(logits, c.s.rows);
   auto loss = at::empty({}, f32), rewards = at::empty({2 * pairs}, f32);
   if (c.s.rows == 0) {
     loss.fill_(0.6931471805599453);
     rewards.zero_();
-    return {loss, rewards, saved};
+    return {loss, rewards};
   }
-  auto partial = at::empty({pairs + 1}, f32.dtype(at::kDouble));
-  double* part = partial.data_ptr<double>();
-  unsigned* ticket = (unsigned*)(part + pairs);
+  const Scratch tmp(logits, pairs, c);
   STOKE_ELEM_SWITCH(logits.scalar_type(), "preference_loss", {
-    auto stats = launch_stats<T>(logits, target, c, ticket);
+    launch_stats<T>(logits, target, c, tmp);
     hipLaunchKernelGGL(
         (prefer_finish_kernel<T>), dim3((unsigned)pairs), dim3(kThreads), 0,
         elem::stream(), (const T*)logits.data_ptr(),
-        target.data_ptr<long>(), (const float2*)stats.data_ptr(),
-        ref_lp.data_ptr<float>(), (float4*)saved.data_ptr(), part, ticket,
+        target.data_ptr<long>(), tmp.stats, ref_lp.data_ptr<float>(),
+        (float4*)saved.data_ptr(), tmp.partial, tmp.ticket,
         loss.data_ptr<float>(), rewards.data_ptr<float>(), c.s, ignore,
         c.pieces, seq, beta, eps);
   });
-  return {loss, rewards, saved};
+  return {loss, rewards};
 }
 
-// up: one value for each row (token_logprobs) or one for all (the losses).
-at::Tensor token_loss_bwd(at::Tensor logits, at::Tensor target,
-                          at::Tensor saved, at::Tensor up,
-                          c10::optional<at::Tensor> scale, int64_t ignore) {
-  const Call c = check(logits, target, ignore, "token_loss");
-  TORCH_CHECK(up.device() == logits.device() && up.is_contiguous() &&
-                  up.scalar_type() == at::kFloat &&
-                  (up.numel() == 1 || up.numel() == c.s.rows),
-              "token_loss: fp32 gradient of one value or one a row required");
-  const c10::DeviceGuard guard(logits.device());
-  auto dlogits = at::empty(logits.sizes(), logits.options());
-  STOKE_ELEM_SWITCH(logits.scalar_type(), "token_loss", {
-    if (c.s.rows > 0)
-      hipLaunchKernelGGL(
-          (lp_bwd_kernel<T>),
-          dim3((unsigned)c.s.rows, (unsigned)c.pieces), dim3(kThreads), 0,
-          elem::stream(), (const T*)logits.data_ptr(),
-          target.data_ptr<long>(), (const float4*)saved.data_ptr(),
-          up.data_ptr<float>(), up.numel() == 1 ? 0 : 1,
-          scale ? scale->data_ptr<float>() : nullptr,
-          (T*)dlogits.data_ptr(), c.s, ignore, c.piece);
-  });
-  return dlogits;
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits,
+                               const at::Tensor& target,
+                               const at::Tensor& ref_lp, double beta,
+                               double eps, int64_t ignore) {
+    at::Tensor saved;
+    auto out = preference_forward(logits, target, ref_lp, beta, eps, ignore,
+                                  saved);
+    ctx->save_for_backward({logits, target, saved});
+    ctx->mark_non_differentiable({out[1]});
+    ctx->saved_data["ignore"] = ignore;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    const auto v = ctx->get_saved_variables();
+    auto d = backward_of(v[0], v[1], (const float4*)v[2].data_ptr(), up[0],
+                         nullptr, ctx->saved_data["ignore"].toInt());
+    variable_list out(6);
+    out[0] = d;
+    return elem::once_differentiable(std::move(out));
+  }
+};
+
+}  // namespace
+
+// The entry points check their arguments and have gradients for the logits.
+at::Tensor token_logprobs(at::Tensor logits, at::Tensor target,
+                          int64_t ignore) {
+  check(logits, target, "token_logprobs");
+  const auto x = rows_of(logits), t = target.contiguous();
+  if (!wants_grad(x)) return logprobs_forward(x, t, ignore, at::Tensor());
+  return TokenLogprobs::apply(x, t, ignore);
+}
+
+at::Tensor policy_loss(at::Tensor logits, at::Tensor target,
+                       at::Tensor old_lp, at::Tensor adv,
+                       std::optional<at::Tensor> ref_lp, double clip_low,
+                       double clip_high, double kl, int64_t ignore) {
+  check(logits, target, "fused_policy_loss");
+  TORCH_CHECK_VALUE(
+      clip_low >= 0 && clip_low <= 1 && clip_high >= 0 && kl >= 0,
+      "Stoke -- fused_policy_loss takes 0 <= clip_low <= 1, clip_high >= 0 "
+      "and kl_coef >= 0, got ", clip_low, ", ", clip_high, ", ", kl);
+  TORCH_CHECK_VALUE(kl == 0 || ref_lp, "Stoke -- kl_coef needs ref_logprobs");
+  const auto x = rows_of(logits), t = target.contiguous();
+  const auto old_rows = per_token(old_lp, target, "old_logprobs");
+  const auto adv_rows = per_token(adv, target, "advantages");
+  std::optional<at::Tensor> ref;
+  if (kl != 0) ref = per_token(*ref_lp, target, "ref_logprobs");
+  if (wants_grad(x))
+    return PolicyLoss::apply(x, t, old_rows, adv_rows, ref, 1. - clip_low,
+                             1. + clip_high, kl, ignore);
+  at::Tensor saved;
+  return policy_forward(x, t, old_rows, adv_rows, ref.value_or(at::Tensor()),
+                        PolicyArgs{1. - clip_low, 1. + clip_high, kl},
+                        ignore, saved);
+}
+
+// (loss, rewards)
+std::vector<at::Tensor> preference_loss(at::Tensor logits, at::Tensor target,
+                                        at::Tensor ref_lp, double beta,
+                                        double eps, int64_t ignore) {
+  check(logits, target, "fused_preference_loss");
+  TORCH_CHECK_VALUE(
+      logits.dim() == 3 && logits.size(0) > 0 && logits.size(0) % 2 == 0,
+      "Stoke -- fused_preference_loss takes logits [2P, S, V] (chosen, then "
+      "rejected), got ", logits.sizes());
+  TORCH_CHECK_VALUE(beta > 0 && eps >= 0 && eps <= 0.5,
+                    "Stoke -- fused_preference_loss takes beta > 0 and "
+                    "0 <= label_smoothing <= 0.5, got ", beta, ", ", eps);
+  const auto x = rows_of(logits), t = target.contiguous();
+  const auto ref = per_token(ref_lp, target, "ref_logprobs");
+  if (wants_grad(x))
+    return PreferenceLoss::apply(x, t, ref, beta, eps, ignore);
+  at::Tensor saved;
+  return preference_forward(x, t, ref, beta, eps, ignore, saved);
 }

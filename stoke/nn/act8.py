@@ -18,6 +18,8 @@ from typing import NamedTuple
 
 import torch
 
+from stoke import ops
+
 _BLOCK = 32
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -75,8 +77,6 @@ def compress_activation(x: torch.Tensor) -> CompressedActivation:
             f"{x.dtype}"
         )
     if x.is_cuda:
-        from stoke import ops
-
         q, scale = ops._require_ext().act8_pack(x.detach().contiguous())
     else:
         q, scale = _eager_pack(x)
@@ -94,8 +94,6 @@ def restore_activation(held: CompressedActivation) -> torch.Tensor:
             "returned: int8 values and one uint8 exponent for every 32"
         )
     if q.is_cuda:
-        from stoke import ops
-
         return ops._require_ext().act8_unpack(q.contiguous(),
                                               scale.contiguous(), dtype)
     return _eager_unpack(q, scale, dtype)
@@ -106,13 +104,6 @@ class _SwiGLU8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, g, u):
-        if g.is_cuda:
-            from stoke import ops
-
-            y, held = ops._require_ext().swiglu8_fwd(g.contiguous(),
-                                                     u.contiguous())
-            ctx.save_for_backward(held)
-            return y
         ctx.save_for_backward(*_eager_pack(g), *_eager_pack(u))
         gf = g.float()
         return (gf * torch.sigmoid(gf) * u.float()).to(g.dtype)
@@ -120,12 +111,6 @@ class _SwiGLU8Fn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        dy = dy.contiguous()
-        if dy.is_cuda:
-            from stoke import ops
-
-            dg, du = ops._require_ext().swiglu8_bwd(dy, *ctx.saved_tensors)
-            return dg, du
         qg, sg, qu, su = ctx.saved_tensors
         g = _eager_unpack(qg, sg, torch.float32)
         u = _eager_unpack(qu, su, torch.float32)
@@ -135,6 +120,9 @@ class _SwiGLU8Fn(torch.autograd.Function):
 
 
 def swiglu8(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+    if g.is_cuda:
+        # the extension checks its arguments in the same way
+        return ops._require_ext().swiglu8(g, u)
     if g.shape != u.shape or g.dtype != u.dtype or g.device != u.device \
             or g.dtype not in _DTYPES:
         raise ValueError(

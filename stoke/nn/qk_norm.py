@@ -18,7 +18,8 @@ from typing import Optional, Sequence, Tuple
 import torch
 import torch.nn as nn
 
-_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+from stoke import ops
+
 _MAX_AXES = 4
 _MAX_DIM = 1024
 
@@ -122,26 +123,6 @@ def _eager(q, k, qw, kw, cos, sin, pos, sections, eps, interleaved):
     return one(q, qw), one(k, kw)
 
 
-class _QKNormRopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, qw, kw, cos, sin, pos, sections, eps, interleaved):
-        from stoke import _C
-
-        ctx.save_for_backward(q, k, qw, kw, cos, sin, pos)
-        ctx.rest = (sections, eps, interleaved)
-        return tuple(_C.qk_norm_rope_fwd(q, k, qw, kw, cos, sin, pos,
-                                         sections, eps, interleaved))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dyq, dyk):
-        from stoke import _C
-
-        grads = _C.qk_norm_rope_bwd(dyq.contiguous(), dyk.contiguous(),
-                                    *ctx.saved_tensors, *ctx.rest)
-        return (*grads, None, None, None, None, None, None)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
                  q_weight: Optional[torch.Tensor],
                  k_weight: Optional[torch.Tensor], cos: torch.Tensor,
@@ -160,26 +141,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     interleaved: pairs (2i, 2i + 1) as ``apply_rope`` has them, else
     (i, i + pairs).  A position outside the tables gives NaN.
     """
+    if q.is_cuda and q.dtype != torch.float64:
+        # the extension checks the arguments as _check does
+        return tuple(ops._require_ext().qk_norm_rope(
+            q, k, q_weight, k_weight, cos, sin, positions, sections, eps,
+            interleaved))
     _check(q, k, q_weight, k_weight, cos, sin, positions, sections)
     if positions is not None:
         positions = positions.expand(*positions.shape[:-2], *q.shape[:2])
-    if not (q.is_cuda and q.dtype in _DTYPES):
-        return _eager(q, k, q_weight, k_weight, cos, sin, positions, sections,
-                      eps, interleaved)
-    from stoke import ops
-
-    ops._require_ext()
-    if q.stride(-1) != 1:
-        q = q.contiguous()
-    if k.stride(-1) != 1:
-        k = k.contiguous()
-    if positions is not None:
-        positions = positions.to(torch.int64).contiguous()
-    return _QKNormRopeFn.apply(
-        q, k, None if q_weight is None else q_weight.contiguous(),
-        None if k_weight is None else k_weight.contiguous(),
-        cos.float().contiguous(), sin.float().contiguous(), positions,
-        list(sections or ()), eps, interleaved)
+    return _eager(q, k, q_weight, k_weight, cos, sin, positions, sections,
+                  eps, interleaved)
 
 
 class StokeQKNorm(nn.Module):

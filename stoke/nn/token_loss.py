@@ -18,14 +18,13 @@ copy.  CPU tensors and float64 take the same formulas in torch.
 
 import torch
 
-_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+from stoke import ops
 
 
 def _native(logits: torch.Tensor):
-    """The extension where the kernels apply, None for the torch formulas."""
-    if logits.is_cuda and logits.dtype in _DTYPES:
-        from stoke import ops
-
+    """The extension where its kernels take the call (it checks the
+    arguments as ``_check`` does), None for the torch formulas."""
+    if logits.is_cuda and logits.dtype != torch.float64:
         return ops._require_ext()
     return None
 
@@ -63,21 +62,6 @@ def _per_token(v, targets, what):
     return v.expand(targets.shape)
 
 
-def _as_3d(logits, targets):
-    if logits.dim() == 2:
-        logits, targets = logits[None], targets[None]
-    elif logits.dim() > 3:
-        logits = logits.flatten(0, -3)
-        targets = targets.flatten(0, -2)
-    if logits.stride(-1) != 1:
-        logits = logits.contiguous()
-    return logits, targets.contiguous()
-
-
-def _rows32(v, targets):
-    return v.to(torch.float32).reshape(targets.shape).contiguous()
-
-
 def _eager_logprobs(logits, targets, ignore_index):
     """(log-probabilities in float64 with zeros where ignored, live)."""
     live = (targets != ignore_index) & (targets >= 0) \
@@ -95,60 +79,18 @@ def _result_dtype(logits):
     return torch.float64 if logits.dtype == torch.float64 else torch.float32
 
 
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, ignore_index):
-        from stoke import _C
-
-        lp, saved = _C.token_logprobs_fwd(logits, targets, ignore_index)
-        ctx.save_for_backward(logits, targets, saved)
-        ctx.ignore_index = ignore_index
-        return lp
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, up):
-        from stoke import _C
-
-        logits, targets, saved = ctx.saved_tensors
-        return _C.token_loss_bwd(logits, targets, saved, up.contiguous(),
-                                 None, ctx.ignore_index), None, None
-
-
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor,
                    ignore_index: int = -100) -> torch.Tensor:
     """log softmax(logits)[targets] in fp32, 0 at ignored positions.
 
     logits: [..., V]; targets: [...] int64.
     """
+    ext = _native(logits)
+    if ext is not None:
+        return ext.token_logprobs(logits, targets, ignore_index)
     _check(logits, targets, "token_logprobs")
-    if _native(logits) is None:
-        lp, _ = _eager_logprobs(logits, targets, ignore_index)
-        return lp.to(_result_dtype(logits))
-    x, t = _as_3d(logits, targets)
-    return _TokenLogprobsFn.apply(x, t, ignore_index).view(targets.shape)
-
-
-class _PolicyLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, old, adv, ref, low, high, kl,
-                ignore_index):
-        from stoke import _C
-
-        loss, saved, inv_count = _C.policy_loss_fwd(
-            logits, targets, old, adv, ref, low, high, kl, ignore_index)
-        ctx.save_for_backward(logits, targets, saved, inv_count)
-        ctx.ignore_index = ignore_index
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, up):
-        from stoke import _C
-
-        logits, targets, saved, inv_count = ctx.saved_tensors
-        return (_C.token_loss_bwd(logits, targets, saved, up, inv_count,
-                                  ctx.ignore_index),) + (None,) * 8
+    lp, _ = _eager_logprobs(logits, targets, ignore_index)
+    return lp.to(_result_dtype(logits))
 
 
 def fused_policy_loss(logits: torch.Tensor, actions: torch.Tensor,
@@ -171,6 +113,11 @@ def fused_policy_loss(logits: torch.Tensor, actions: torch.Tensor,
     token left the loss and its gradient are 0.  ``ref_logprobs`` is
     required where ``kl_coef`` is not 0.
     """
+    ext = _native(logits)
+    if ext is not None:
+        return ext.policy_loss(logits, actions, old_logprobs, advantages,
+                               ref_logprobs, clip_low, clip_high, kl_coef,
+                               ignore_index)
     _check(logits, actions, "fused_policy_loss")
     if not (0 <= clip_low <= 1 and clip_high >= 0 and kl_coef >= 0):
         raise ValueError(
@@ -178,55 +125,21 @@ def fused_policy_loss(logits: torch.Tensor, actions: torch.Tensor,
             f"clip_high >= 0 and kl_coef >= 0, got {clip_low}, {clip_high}, "
             f"{kl_coef}"
         )
-    if kl_coef == 0:
-        ref_logprobs = None
-    elif ref_logprobs is None:
+    if kl_coef != 0 and ref_logprobs is None:
         raise ValueError("Stoke -- kl_coef needs ref_logprobs")
     old = _per_token(old_logprobs, actions, "old_logprobs")
     adv = _per_token(advantages, actions, "advantages")
-    ref = ref_logprobs
-    if ref is not None:
-        ref = _per_token(ref, actions, "ref_logprobs")
-    low, high = 1.0 - clip_low, 1.0 + clip_high
-    if _native(logits) is None:
-        lp, live = _eager_logprobs(logits, actions, ignore_index)
-        lp, adv = lp[live], adv[live].double()
-        rho = (lp - old[live].double()).exp()
-        free, held = rho * adv, rho.clamp(low, high) * adv
-        # torch.minimum halves the gradient where both are the same
-        tok = -torch.where(free > held, held, free)
-        if ref is not None:
-            d = ref[live].double() - lp
-            tok = tok + kl_coef * (d.exp() - d - 1)
-        loss = tok.sum() / max(1, tok.numel())
-        return loss.to(_result_dtype(logits))
-    x, t = _as_3d(logits, actions)
-    return _PolicyLossFn.apply(
-        x, t, _rows32(old, t), _rows32(adv, t),
-        None if ref is None else _rows32(ref, t), low, high, kl_coef,
-        ignore_index)
-
-
-class _PreferenceLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, ref, beta, smoothing, ignore_index):
-        from stoke import _C
-
-        loss, rewards, saved = _C.preference_loss_fwd(
-            logits, targets, ref, beta, smoothing, ignore_index)
-        ctx.save_for_backward(logits, targets, saved)
-        ctx.mark_non_differentiable(rewards)
-        ctx.ignore_index = ignore_index
-        return loss, rewards
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, up, _):
-        from stoke import _C
-
-        logits, targets, saved = ctx.saved_tensors
-        return (_C.token_loss_bwd(logits, targets, saved, up, None,
-                                  ctx.ignore_index),) + (None,) * 5
+    lp, live = _eager_logprobs(logits, actions, ignore_index)
+    lp, adv = lp[live], adv[live].double()
+    rho = (lp - old[live].double()).exp()
+    free, held = rho * adv, rho.clamp(1 - clip_low, 1 + clip_high) * adv
+    # torch.minimum halves the gradient where both are the same
+    tok = -torch.where(free > held, held, free)
+    if kl_coef != 0:
+        ref = _per_token(ref_logprobs, actions, "ref_logprobs")
+        d = ref[live].double() - lp
+        tok = tok + kl_coef * (d.exp() - d - 1)
+    return (tok.sum() / max(1, tok.numel())).to(_result_dtype(logits))
 
 
 def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
@@ -246,6 +159,10 @@ def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
 
     and the loss the mean over the pairs.
     """
+    ext = _native(logits)
+    if ext is not None:
+        return tuple(ext.preference_loss(logits, targets, ref_logprobs, beta,
+                                         label_smoothing, ignore_index))
     _check(logits, targets, "fused_preference_loss")
     if logits.dim() != 3 or logits.shape[0] % 2 or logits.shape[0] == 0:
         raise ValueError(
@@ -258,16 +175,12 @@ def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
             f"0 <= label_smoothing <= 0.5, got {beta}, {label_smoothing}"
         )
     ref = _per_token(ref_logprobs, targets, "ref_logprobs")
-    if _native(logits) is None:
-        lp, live = _eager_logprobs(logits, targets, ignore_index)
-        gap = torch.where(live, lp - ref.double().masked_fill(~live, 0.0), 0.0)
-        rewards = beta * gap.sum(-1)
-        good, bad = rewards.chunk(2)
-        h = good - bad
-        ls = torch.nn.functional.logsigmoid
-        loss = -((1 - label_smoothing) * ls(h) + label_smoothing * ls(-h))
-        dt = _result_dtype(logits)
-        return loss.mean().to(dt), rewards.detach().to(dt)
-    x, t = _as_3d(logits, targets)
-    return _PreferenceLossFn.apply(x, t, _rows32(ref, t), beta,
-                                   label_smoothing, ignore_index)
+    lp, live = _eager_logprobs(logits, targets, ignore_index)
+    gap = torch.where(live, lp - ref.double().masked_fill(~live, 0.0), 0.0)
+    rewards = beta * gap.sum(-1)
+    good, bad = rewards.chunk(2)
+    h = good - bad
+    ls = torch.nn.functional.logsigmoid
+    loss = -((1 - label_smoothing) * ls(h) + label_smoothing * ls(-h))
+    dt = _result_dtype(logits)
+    return loss.mean().to(dt), rewards.detach().to(dt)

@@ -125,27 +125,31 @@ def test_empty_and_strided_and_offset_inputs(device):
         assert torch.equal(a.scales, b.scales)
 
 
-def test_refusals():
-    with pytest.raises(ValueError):
-        compress_activation(torch.zeros(4, dtype=torch.float64))
-    held = compress_activation(torch.zeros(40))
-    with pytest.raises(ValueError):
-        restore_activation(CompressedActivation(
-            held.values, held.scales[:1], held.dtype))
-    with pytest.raises(ValueError):
-        restore_activation(CompressedActivation(
-            held.values.float(), held.scales, held.dtype))
-    with pytest.raises(ValueError):
-        restore_activation(CompressedActivation(
-            held.values, held.scales, torch.int32))
-    with pytest.raises(ValueError):
-        swiglu(torch.zeros(4), torch.zeros(4), save_bits=4)
-    with pytest.raises(ValueError):
-        swiglu(torch.zeros(4, 4), torch.zeros(4), save_bits=8)
-    with pytest.raises(ValueError):
-        swiglu(torch.zeros(4), torch.zeros(4).half(), save_bits=8)
-    with pytest.raises(ValueError):
-        apply_activation_checkpointing(torch.nn.Linear(2, 2), save_bits=12)
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    _skip(device)
+    def zeros(*shape, dtype=torch.float32):
+        return torch.zeros(*shape, dtype=dtype, device=device)
+
+    held = compress_activation(zeros(40))
+    cases = [
+        lambda: compress_activation(zeros(4, dtype=torch.float64)),
+        lambda: restore_activation(CompressedActivation(
+            held.values, held.scales[:1], held.dtype)),
+        lambda: restore_activation(CompressedActivation(
+            held.values.float(), held.scales, held.dtype)),
+        lambda: restore_activation(CompressedActivation(
+            held.values, held.scales, torch.int32)),
+        lambda: swiglu(zeros(4), zeros(4), save_bits=4),
+        lambda: swiglu(zeros(4, 4), zeros(4), save_bits=8),
+        lambda: swiglu(zeros(4), zeros(4).half(), save_bits=8),
+        lambda: swiglu(zeros(4).double(), zeros(4).double(), save_bits=8),
+        lambda: apply_activation_checkpointing(
+            torch.nn.Linear(2, 2), save_bits=12),
+    ]
+    for call in cases:
+        with pytest.raises(ValueError):
+            call()
 
 
 # ------------------------------------------------------------------ SwiGLU

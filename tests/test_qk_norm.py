@@ -271,9 +271,11 @@ def test_gradients_against_differences():
                 sections=sec, interleaved=inter), (q, k, qw, kw))
 
 
-def test_refusals():
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    _skip(device)
     (q, k, qw, kw, cos, sin, pos, _, _), _ = _case(
-        2, 6, 3, 1, 64, 64, torch.float32, torch.float32)
+        2, 6, 3, 1, 64, 64, torch.float32, torch.float32, device=device)
     ok = dict(positions=pos)
     pos3 = pos.expand(3, 2, 6)
     cases = [

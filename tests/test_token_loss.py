@@ -353,9 +353,12 @@ def test_gradients_against_differences():
         assert torch.autograd.gradcheck(fn, (x.requires_grad_(True),))
 
 
-def test_refusals():
-    x, t = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64)
-    v = torch.zeros(2, 3)
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    _skip(device)
+    x = torch.zeros(2, 3, 5, device=device)
+    t = torch.zeros(2, 3, dtype=torch.int64, device=device)
+    v = torch.zeros(2, 3, device=device)
     cases = [
         lambda: token_logprobs(x, t.int()),
         lambda: token_logprobs(x, t[:, :2]),
@@ -447,3 +450,17 @@ def test_gpu_on_another_stream():
     z = x.clone().requires_grad_(True)
     gz, = torch.autograd.grad(token_logprobs(z, t).sum(), z)
     assert torch.equal(g, gz)
+
+
+@pytest.mark.gpu
+def test_gpu_second_derivative_is_refused():
+    _skip("cuda")
+    x, t = _inputs((2, 3, 50), torch.float32, "cuda", keep=1.0)
+    x.requires_grad_(True)
+    v = torch.zeros(2, 3, device="cuda")
+    for loss in (token_logprobs(x, t).sum(),
+                 fused_policy_loss(x, t, v, v + 1),
+                 fused_preference_loss(x, t, v)[0]):
+        g, = torch.autograd.grad(loss, x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.square().sum().backward()
