@@ -104,21 +104,21 @@ __device__ __forceinline__ void unpack_run(const Bytes q, unsigned exp,
   }
 }
 
-template <typename T>
+template <bool NT, typename T>
 __device__ __forceinline__ void load_run(const T* __restrict__ p, long i,
                                          float (&v)[kRun]) {
-  const Run<T> w = *(const Run<T>*)(p + i);
+  const Run<T> w = elem::load<NT>((const Run<T>*)(p + i));
   #pragma unroll
   for (int e = 0; e < kRun; ++e) v[e] = (float)w[e];
 }
 
-template <typename T>
+template <bool NT, typename T>
 __device__ __forceinline__ void store_run(T* __restrict__ p, long i,
                                           const float (&v)[kRun]) {
   Run<T> w;
   #pragma unroll
   for (int e = 0; e < kRun; ++e) w[e] = (T)v[e];
-  *(Run<T>*)(p + i) = w;
+  elem::store<NT>((Run<T>*)(p + i), w);
 }
 
 __device__ __forceinline__ float sigmoid(float a) {
@@ -142,7 +142,10 @@ __device__ __forceinline__ void swiglu_grad(float d, float a, float b,
 // two 16-byte) accesses for the whole blocks of 32; the last, partial block
 // and tensors that do not start on 16 bytes go one value a thread.  `first`
 // is where the second form begins, a multiple of 32.
-template <typename T>
+// NT: tensors over elem::kCached are read past the caches (and, in the
+// backward, written).  What the forward writes is read by the next product:
+// it goes through them.
+template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void pack_kernel(
     const T* __restrict__ x, signed char* __restrict__ q,
     unsigned char* __restrict__ scale, long n, long first) {
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(
   for (long i = me * kRun; i < first; i += step * kRun) {
     float v[kRun];
     Bytes b;
-    load_run(x, i, v);
+    load_run<NT>(x, i, v);
     const unsigned e = pack_run(v, b);
     *(Bytes*)(q + i) = b;
     if ((threadIdx.x & 3) == 0) scale[i >> 5] = (unsigned char)e;
@@ -166,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(
   }
 }
 
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void unpack_kernel(
     const signed char* __restrict__ q,
     const unsigned char* __restrict__ scale, T* __restrict__ x, long n,
@@ -175,15 +178,15 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(
   const long me = (long)blockIdx.x * kThreads + threadIdx.x;
   for (long i = me * kRun; i < first; i += step * kRun) {
     float v[kRun];
-    unpack_run<T>(*(const Bytes*)(q + i), scale[i >> 5], v);
-    store_run(x, i, v);
+    unpack_run<T>(elem::load<NT>((const Bytes*)(q + i)), scale[i >> 5], v);
+    store_run<false>(x, i, v);
   }
   for (long i = first + me; i < n; i += step)
     x[i] = (T)restored<T>(q[i], scale[i >> 5]);
 }
 
 // y = silu(g) * u from the values as they come; g and u stay in 8 bits.
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     const T* __restrict__ g, const T* __restrict__ u, T* __restrict__ y,
     signed char* __restrict__ qg, signed char* __restrict__ qu,
@@ -193,13 +196,13 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
   const long me = (long)blockIdx.x * kThreads + threadIdx.x;
   for (long i = me * kRun; i < first; i += step * kRun) {
     float a[kRun], b[kRun], o[kRun];
-    load_run(g, i, a);
-    load_run(u, i, b);
+    load_run<NT>(g, i, a);
+    load_run<NT>(u, i, b);
     Bytes qa, qb;
     const unsigned ea = pack_run(a, qa), eb = pack_run(b, qb);
     #pragma unroll
     for (int e = 0; e < kRun; ++e) o[e] = swiglu(a[e], b[e]);
-    store_run(y, i, o);
+    store_run<false>(y, i, o);
     *(Bytes*)(qg + i) = qa;
     *(Bytes*)(qu + i) = qb;
     if ((threadIdx.x & 3) == 0) {
@@ -227,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
   }
 }
 
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void swiglu8_bwd_kernel(
     const T* __restrict__ dy, const signed char* __restrict__ qg,
     const signed char* __restrict__ qu, const unsigned char* __restrict__ sg,
@@ -237,14 +240,14 @@ __global__ __launch_bounds__(kThreads) void swiglu8_bwd_kernel(
   const long me = (long)blockIdx.x * kThreads + threadIdx.x;
   for (long i = me * kRun; i < first; i += step * kRun) {
     float d[kRun], a[kRun], b[kRun], da[kRun], db[kRun];
-    load_run(dy, i, d);
-    unpack_run<T>(*(const Bytes*)(qg + i), sg[i >> 5], a);
-    unpack_run<T>(*(const Bytes*)(qu + i), su[i >> 5], b);
+    load_run<NT>(dy, i, d);
+    unpack_run<T>(elem::load<NT>((const Bytes*)(qg + i)), sg[i >> 5], a);
+    unpack_run<T>(elem::load<NT>((const Bytes*)(qu + i)), su[i >> 5], b);
     #pragma unroll
     for (int e = 0; e < kRun; ++e)
       swiglu_grad(d[e], a[e], b[e], da[e], db[e]);
-    store_run(dg, i, da);
-    store_run(du, i, db);
+    store_run<NT>(dg, i, da);
+    store_run<NT>(du, i, db);
   }
   for (long i = first + me; i < n; i += step) {
     float da, db;
@@ -261,10 +264,17 @@ long first_of(long n, P... p) {
   return (elem::aligned16(p) && ...) ? n / 32 * 32 : 0;
 }
 
-inline dim3 grid_for(long n, long first) {
-  const long threads = std::max(first / kRun, n - first);
+inline dim3 grid_for(long n, long first, int runs = 1) {
+  const long threads = std::max(first / kRun / runs, n - first);
   return dim3((unsigned)std::min<long>((threads + kThreads - 1) / kThreads,
                                        1 << 20));
+}
+
+// Calls f with whether the accesses go past the caches as a constant.
+template <typename F>
+void with_caching(long bytes, F f) {
+  if (bytes > elem::kCached) f(std::true_type{});
+  else f(std::false_type{});
 }
 
 // Pieces of the byte buffer that holds g and u: both values, then both
@@ -298,10 +308,12 @@ at::Tensor swiglu8_forward(const at::Tensor& g, const at::Tensor& u,
   const Held h(held.data_ptr(), n);
   STOKE_ELEM_SWITCH(g.scalar_type(), "swiglu8", {
     const long first = first_of(n, g.data_ptr(), u.data_ptr());
-    hipLaunchKernelGGL((swiglu8_fwd_kernel<T>), grid_for(n, first),
-                       dim3(kThreads), 0, elem::stream(),
-                       (const T*)g.data_ptr(), (const T*)u.data_ptr(),
-                       (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first);
+    with_caching(n * (long)sizeof(T), [&](auto nt) {
+      hipLaunchKernelGGL((swiglu8_fwd_kernel<T, nt>), grid_for(n, first),
+                         dim3(kThreads), 0, elem::stream(),
+                         (const T*)g.data_ptr(), (const T*)u.data_ptr(),
+                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first);
+    });
   });
   return y;
 }
@@ -315,10 +327,12 @@ variable_list swiglu8_backward(const at::Tensor& dy, const at::Tensor& held) {
   const Held h(held.data_ptr(), n);
   STOKE_ELEM_SWITCH(dy.scalar_type(), "swiglu8", {
     const long first = first_of(n, dy.data_ptr());
-    hipLaunchKernelGGL((swiglu8_bwd_kernel<T>), grid_for(n, first),
-                       dim3(kThreads), 0, elem::stream(),
-                       (const T*)dy.data_ptr(), h.qg, h.qu, h.sg, h.su,
-                       (T*)dg.data_ptr(), (T*)du.data_ptr(), n, first);
+    with_caching(n * (long)sizeof(T), [&](auto nt) {
+      hipLaunchKernelGGL((swiglu8_bwd_kernel<T, nt>), grid_for(n, first),
+                         dim3(kThreads), 0, elem::stream(),
+                         (const T*)dy.data_ptr(), h.qg, h.qu, h.sg, h.su,
+                         (T*)dg.data_ptr(), (T*)du.data_ptr(), n, first);
+    });
   });
   return {dg, du};
 }
@@ -349,11 +363,15 @@ std::vector<at::Tensor> act8_pack(at::Tensor x) {
   auto scale = at::empty({(n + 31) / 32}, x.options().dtype(at::kByte));
   STOKE_ELEM_SWITCH(x.scalar_type(), "act8_pack", {
     const long first = first_of(n, x.data_ptr());
+    // past the caches a thread takes two runs: 134M values 63 against 67 us
     if (n > 0)
-      hipLaunchKernelGGL((pack_kernel<T>), grid_for(n, first),
-                         dim3(kThreads), 0, elem::stream(),
-                         (const T*)x.data_ptr(), (signed char*)q.data_ptr(),
-                         (unsigned char*)scale.data_ptr(), n, first);
+      with_caching(n * (long)sizeof(T), [&](auto nt) {
+        hipLaunchKernelGGL((pack_kernel<T, nt>),
+                           grid_for(n, first, nt ? 2 : 1), dim3(kThreads), 0,
+                           elem::stream(), (const T*)x.data_ptr(),
+                           (signed char*)q.data_ptr(),
+                           (unsigned char*)scale.data_ptr(), n, first);
+      });
   });
   return {q, scale};
 }
@@ -372,11 +390,13 @@ at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype) {
   STOKE_ELEM_SWITCH(dtype, "act8_unpack", {
     const long first = first_of(n, q.data_ptr());
     if (n > 0)
-      hipLaunchKernelGGL((unpack_kernel<T>), grid_for(n, first),
-                         dim3(kThreads), 0, elem::stream(),
-                         (const signed char*)q.data_ptr(),
-                         (const unsigned char*)scale.data_ptr(),
-                         (T*)x.data_ptr(), n, first);
+      with_caching(n * (long)sizeof(T), [&](auto nt) {
+        hipLaunchKernelGGL((unpack_kernel<T, nt>),
+                           grid_for(n, first, nt ? 2 : 1), dim3(kThreads), 0,
+                           elem::stream(), (const signed char*)q.data_ptr(),
+                           (const unsigned char*)scale.data_ptr(),
+                           (T*)x.data_ptr(), n, first);
+      });
   });
   return x;
 }

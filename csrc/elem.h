@@ -18,22 +18,24 @@ using vec = T __attribute__((ext_vector_type(N)));
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// A 16-byte access, past the caches where NT is set.
+// Vector accesses, past the caches where NT is set.
 template <bool NT, typename V>
-__device__ __forceinline__ V load16(const V* p) {
-  static_assert(sizeof(V) == 16);
+__device__ __forceinline__ V load(const V* p) {
+  using Words = vec<int, sizeof(V) / 4>;
   if (!NT) return *p;
-  return __builtin_bit_cast(
-      V, __builtin_nontemporal_load((const vec<int, 4>*)p));
+  return __builtin_bit_cast(V, __builtin_nontemporal_load((const Words*)p));
 }
 template <bool NT, typename V>
-__device__ __forceinline__ void store16(V* p, const V& v) {
-  static_assert(sizeof(V) == 16);
+__device__ __forceinline__ void store(V* p, const V& v) {
+  using Words = vec<int, sizeof(V) / 4>;
   if (!NT) *p = v;
   else
-    __builtin_nontemporal_store(__builtin_bit_cast(vec<int, 4>, v),
-                                (vec<int, 4>*)p);
+    __builtin_nontemporal_store(__builtin_bit_cast(Words, v), (Words*)p);
 }
+
+// Tensors up to this size stay in the 256 MB last-level cache next to what is
+// made of them; larger ones go past it.
+constexpr long kCached = 128L << 20;
 
 inline hipStream_t stream() {
   return at::hip::getCurrentHIPStream().stream();

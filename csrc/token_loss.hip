@@ -383,7 +383,7 @@ __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
   if (c == 0.f) {
     const Vec zero = (Vec)(T)0.f;
     for (int i = threadIdx.x; i < body; i += THREADS)
-      elem::store16<NT>(dv + i, zero);
+      elem::store<NT>(dv + i, zero);
     if ((int)threadIdx.x < rest) dx[lone] = (T)0.f;
     return;
   }
@@ -405,13 +405,13 @@ __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
       Vec w[4];
       #pragma unroll
       for (int u = 0; u < 4; ++u)
-        w[u] = elem::load16<NT>(xv + i + u * THREADS);
+        w[u] = elem::load<NT>(xv + i + u * THREADS);
       #pragma unroll
       for (int u = 0; u < 4; ++u)
-        elem::store16<NT>(dv + i + u * THREADS, slope(w[u]));
+        elem::store<NT>(dv + i + u * THREADS, slope(w[u]));
     }
     for (; i < body; i += THREADS)
-      elem::store16<NT>(dv + i, slope(elem::load16<NT>(xv + i)));
+      elem::store<NT>(dv + i, slope(elem::load<NT>(xv + i)));
     if ((int)threadIdx.x < rest)
       dx[lone] = (T)(k * exp_neg((float)x[lone] - r.x));
   } else {
@@ -540,13 +540,6 @@ void launch_stats(const at::Tensor& logits, const at::Tensor& target,
                      c.pieces, c.piece, nullptr, nullptr);
 }
 
-// Logits and gradient of up to this size each stay in the 256 MB last-level
-// cache, where the next product finds the gradient.  Larger ones go past it
-// in the backward, which leaves there what the forward read last: 8192 x
-// 128256 bf16, 60 % of the rows read, forward and backward 790 us against
-// 900 us through the caches; at 512 rows (131 MB) 52 against 50 us.
-constexpr long kCached = 128L << 20;
-
 // dlogits of a loss with `saved` row statistics.  up: one value for each row
 // (token_logprobs) or one for all (the losses).
 at::Tensor backward_of(const at::Tensor& logits, const at::Tensor& target,
@@ -573,7 +566,12 @@ at::Tensor backward_of(const at::Tensor& logits, const at::Tensor& target,
         launch(std::integral_constant<int, kThreads>{}, past_caches);
     };
     if (c.s.rows > 0) {
-      if (c.s.rows * c.s.vocab * (long)sizeof(T) > kCached)
+      // the next product reads the gradient: where it fits, it stays in the
+      // last-level cache.  Past it the backward leaves there what the
+      // forward read last: 8192 x 128256 bf16, 60 % of the rows read,
+      // forward and backward 790 us against 900 us through the caches; at
+      // 512 rows (131 MB) 52 against 50 us.
+      if (c.s.rows * c.s.vocab * (long)sizeof(T) > elem::kCached)
         sized(std::true_type{});
       else
         sized(std::false_type{});
