@@ -201,6 +201,13 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
 // 64 / G heads of one token at a time and goes through the token's heads of
 // queries, then keys.  The angles and positions of a token are read once.
 // Needs 16-byte rows: D, strides and pairs in multiples of 8 (see fits()).
+//
+// Bound by memory.  Heads of more than elem::kCached are written past the
+// caches (NT): 16384 tokens of 32 + 8 heads of 128 in bf16 take 58 us forward
+// (336 MB, 5.7 TB/s; 66 us through the caches) and 90 + 4 us backward
+// (503 MB, 5.6 TB/s; 110 us).  The backward keeps dw in registers over all
+// rows of a wave; 1024 blocks hide its latency (512: 126 us) and more of them
+// only lengthen the sum over blocks (4096: 10 us).
 constexpr int kRun = 8;
 
 template <typename T>
@@ -341,7 +348,7 @@ __device__ __forceinline__ Item item_of(const Args& a, long item, int chunks,
   return it;
 }
 
-template <typename T, int G, bool INTER>
+template <typename T, int G, bool INTER, bool NT>
 __device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
                                          const Lane& l, const Item& it,
                                          int h0, int h1,
@@ -382,12 +389,12 @@ __device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
       Run<T> out;
       #pragma unroll
       for (int e = 0; e < kRun; ++e) out[e] = (T)o[e];
-      *(Run<T>*)(y + (long)h * a.dim) = out;
+      elem::store<NT>((Run<T>*)(y + (long)h * a.dim), out);
     }
   }
 }
 
-template <typename T, int G, bool INTER>
+template <typename T, int G, bool INTER, bool NT>
 __global__ __launch_bounds__(kThreads) void fwd_rows_kernel(Args a,
                                                             int chunks,
                                                             int per) {
@@ -408,14 +415,14 @@ __global__ __launch_bounds__(kThreads) void fwd_rows_kernel(Args a,
     const Item it = item_of(a, i, chunks, per);
     float c[P], sn[P];
     angles<INTER>(a, l, it.token, it.in_seq, c, sn);
-    fwd_side<T, G, INTER>(a, a.side[0], l, it, it.h0, min(it.h1, hq), wq,
+    fwd_side<T, G, INTER, NT>(a, a.side[0], l, it, it.h0, min(it.h1, hq), wq,
                           woq, c, sn);
-    fwd_side<T, G, INTER>(a, a.side[1], l, it, max(it.h0 - hq, 0),
+    fwd_side<T, G, INTER, NT>(a, a.side[1], l, it, max(it.h0 - hq, 0),
                           it.h1 - hq, wk, wok, c, sn);
   }
 }
 
-template <typename T, int G, bool INTER>
+template <typename T, int G, bool INTER, bool NT>
 __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
                                          const Lane& l, const Item& it,
                                          int h0, int h1,
@@ -465,12 +472,12 @@ __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
       out[e] = (T)(r * (dn[e] * w[e] - v[e] * k));
       dw[e] += dn[e] * v[e] * r;
     }
-    if (l.on) *(Run<T>*)(dx + (long)h * a.dim) = out;
+    if (l.on) elem::store<NT>((Run<T>*)(dx + (long)h * a.dim), out);
   }
 }
 
 // partial[block]: dw of the queries, then of the keys.
-template <typename T, int G, bool INTER>
+template <typename T, int G, bool INTER, bool NT>
 __global__ __launch_bounds__(kThreads) void bwd_rows_kernel(
     Args a, int chunks, int per, float* __restrict__ partial) {
   constexpr int P = INTER ? kRun / 2 : kRun;
@@ -489,9 +496,9 @@ __global__ __launch_bounds__(kThreads) void bwd_rows_kernel(
     const Item it = item_of(a, i, chunks, per);
     float c[P], sn[P];
     angles<INTER>(a, l, it.token, it.in_seq, c, sn);
-    bwd_side<T, G, INTER>(a, a.side[0], l, it, it.h0, min(it.h1, hq), w[0],
+    bwd_side<T, G, INTER, NT>(a, a.side[0], l, it, it.h0, min(it.h1, hq), w[0],
                           dw[0], c, sn);
-    bwd_side<T, G, INTER>(a, a.side[1], l, it, max(it.h0 - hq, 0),
+    bwd_side<T, G, INTER, NT>(a, a.side[1], l, it, max(it.h0 - hq, 0),
                           it.h1 - hq, w[1], dw[1], c, sn);
   }
   if (!partial) return;
@@ -633,7 +640,7 @@ void share(const Args& a, long most, int& q_blocks, int& blocks) {
 }
 
 // Whether the kernels with rows in registers take the call.
-bool fits(const Args& a, size_t elem) {
+bool fits(const Args& a, size_t size) {
   if (a.dim % kRun || a.dim > 64 * kRun) return false;
   if (a.half % (a.interleaved ? kRun / 2 : kRun)) return false;
   if (!elem::aligned16(a.cosines) || !elem::aligned16(a.sines)) return false;
@@ -641,7 +648,7 @@ bool fits(const Args& a, size_t elem) {
     if (!elem::aligned16(s.x) || !elem::aligned16(s.dy) ||
         !elem::aligned16(s.w))
       return false;
-    const long step = 16 / (long)elem;
+    const long step = 16 / (long)size;
     if (s.sb % step || s.ss % step || s.sh % step) return false;
   }
   return true;
@@ -659,17 +666,24 @@ void divide(const Args& a, int lanes, int& chunks, int& per) {
   chunks = (int)((heads + per - 1) / per);
 }
 
-// Calls f with the lanes of a row and the pair layout as constants.
+// Calls f with the lanes of a row, the pair layout and the way to memory as
+// constants.
 template <typename F>
-void with_layout(const Args& a, F f) {
-  auto inter = [&](auto lanes) {
-    if (a.interleaved) f(lanes, std::true_type{});
-    else f(lanes, std::false_type{});
+void with_layout(const Args& a, size_t size, F f) {
+  const long bytes = a.tokens * (a.side[0].heads + a.side[1].heads) * a.dim *
+                     (long)size;
+  const auto cached = [&](auto lanes, auto inter) {
+    if (bytes > elem::kCached) f(lanes, inter, std::true_type{});
+    else f(lanes, inter, std::false_type{});
   };
-  if (a.dim <= 8 * kRun) inter(std::integral_constant<int, 8>{});
-  else if (a.dim <= 16 * kRun) inter(std::integral_constant<int, 16>{});
-  else if (a.dim <= 32 * kRun) inter(std::integral_constant<int, 32>{});
-  else inter(std::integral_constant<int, 64>{});
+  const auto layout = [&](auto lanes) {
+    if (a.interleaved) cached(lanes, std::true_type{});
+    else cached(lanes, std::false_type{});
+  };
+  if (a.dim <= 8 * kRun) layout(std::integral_constant<int, 8>{});
+  else if (a.dim <= 16 * kRun) layout(std::integral_constant<int, 16>{});
+  else if (a.dim <= 32 * kRun) layout(std::integral_constant<int, 32>{});
+  else layout(std::integral_constant<int, 64>{});
 }
 
 using torch::autograd::AutogradContext;
@@ -683,11 +697,11 @@ variable_list forward_of(const Tensors& t, const Mode& m) {
   if (a.tokens * (a.side[0].heads + a.side[1].heads) == 0) return {yq, yk};
   STOKE_ELEM_SWITCH(t.q.scalar_type(), "qk_norm_rope", {
     if (fits(a, sizeof(T))) {
-      with_layout(a, [&](auto lanes, auto inter) {
+      with_layout(a, sizeof(T), [&](auto lanes, auto inter, auto nt) {
         int chunks, per;
         divide(a, lanes, chunks, per);
         const long blocks = (a.tokens * chunks + kWaves - 1) / kWaves;
-        hipLaunchKernelGGL((fwd_rows_kernel<T, lanes, inter>),
+        hipLaunchKernelGGL((fwd_rows_kernel<T, lanes, inter, nt>),
                            dim3((unsigned)std::min(blocks, 1L << 20)),
                            dim3(kThreads), 0, elem::stream(), a, chunks, per);
       });
@@ -725,14 +739,14 @@ variable_list backward_of(const Tensors& t, const Mode& m,
   const auto f32 = t.q.options().dtype(at::kFloat);
   STOKE_ELEM_SWITCH(t.q.scalar_type(), "qk_norm_rope", {
     if (fits(a, sizeof(T))) {
-      with_layout(a, [&](auto lanes, auto inter) {
+      with_layout(a, sizeof(T), [&](auto lanes, auto inter, auto nt) {
         int chunks, per;
         divide(a, lanes, chunks, per);
         const long blocks =
             std::min((a.tokens * chunks + kWaves - 1) / kWaves, 1024L);
         at::Tensor partial;
         if (sums) partial = at::empty({blocks, 2 * a.dim}, f32);
-        hipLaunchKernelGGL((bwd_rows_kernel<T, lanes, inter>),
+        hipLaunchKernelGGL((bwd_rows_kernel<T, lanes, inter, nt>),
                            dim3((unsigned)blocks), dim3(kThreads), 0,
                            elem::stream(), a, chunks, per,
                            sums ? partial.data_ptr<float>() : nullptr);
