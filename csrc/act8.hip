@@ -411,5 +411,6 @@ at::Tensor swiglu8(at::Tensor g, at::Tensor u) {
       "Stoke -- swiglu(save_bits=8) takes gate and up of one shape, device "
       "and dtype (bf16, fp16, fp32), got ", g.sizes(), " ", g.scalar_type(),
       " and ", u.sizes(), " ", u.scalar_type());
+  if (at::GradMode::is_enabled()) elem::check_capture({g, u});
   return SwiGLU8::apply(g, u);
 }

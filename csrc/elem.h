@@ -7,6 +7,8 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 namespace elem {
@@ -43,6 +45,27 @@ inline hipStream_t stream() {
 
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// A leaf's gradient belongs to the stream on which a graph first reached it,
+// for as long as any graph that does lives.  A backward captured elsewhere
+// would wait there on an event of the capture, which ends the process: such a
+// call is refused in the forward, before anything is recorded.
+inline void check_capture(std::initializer_list<at::Tensor> inputs) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() ==
+      c10::hip::CaptureStatus::None)
+    return;
+  for (const at::Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    const auto at = node->stream();
+    const c10::impl::VirtualGuardImpl guard(t.device().type());
+    TORCH_CHECK(!at || *at == guard.getStream(t.device()),
+                "Stoke -- a graph capture with gradients of a leaf that an "
+                "autograd graph of another stream still holds: drop that "
+                "graph (its outputs and losses) before the capture");
+  }
 }
 
 // Gradients of a kernel without a derivative of its own: a second backward

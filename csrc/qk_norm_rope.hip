@@ -51,10 +51,11 @@ __device__ __forceinline__ float weight(const Side& s, bool fp32, int e) {
 }
 
 // Cosine and sine of pair p at a token.
-__device__ __forceinline__ float2 angle(const Args& a, long token, int p) {
+__device__ __forceinline__ float2 angle(const Args& a, long token,
+                                        long in_seq, int p) {
   int axis = 0;
   while (axis + 1 < a.axes && p >= a.ends[axis]) ++axis;
-  const long at = a.pos ? a.pos[axis * a.tokens + token] : token % a.seq;
+  const long at = a.pos ? a.pos[axis * a.tokens + token] : in_seq;
   if (at < 0 || at >= a.table) {
     const float nan = __uint_as_float(0x7fc00000);
     return make_float2(nan, nan);
@@ -68,12 +69,19 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-template <typename T>
-__device__ __forceinline__ const T* row_of(const Args& a, const Side& s,
-                                           long row) {
-  const long token = row / s.heads;
-  return (const T*)s.x + (token / a.seq) * s.sb + (token % a.seq) * s.ss +
-         (row % s.heads) * s.sh;
+// Where a row lies.
+struct Row {
+  long token, in_seq, offset;  // of x
+};
+
+__device__ __forceinline__ Row row_of(const Args& a, const Side& s,
+                                      long row) {
+  Row r;
+  r.token = row / s.heads;
+  const long no = r.token / a.seq;
+  r.in_seq = r.token - no * a.seq;
+  r.offset = no * s.sb + r.in_seq * s.ss + (row - r.token * s.heads) * s.sh;
+  return r;
 }
 
 // The other value of e's pair.
@@ -105,9 +113,10 @@ __global__ __launch_bounds__(kThreads) void fwd_any_kernel(Args a,
   for (long base = block * kWaves; base < total; base += blocks * kWaves) {
     const long row = base + wave;
     const bool live = row < total;
+    const Row at = row_of(a, s, live ? row : 0);
     float r = 0.f;
     if (live) {
-      const T* x = row_of<T>(a, s, row);
+      const T* x = (const T*)s.x + at.offset;
       float sum = 0.f;
       for (int e = lane; e < a.dim; e += 64) {
         const float v = (float)x[e];
@@ -122,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void fwd_any_kernel(Args a,
       for (int e = lane; e < a.dim; e += 64) {
         float v = mine[e] * r;
         if (e < 2 * a.half) {
-          const float2 cs = angle(a, row / s.heads, pair_of(a, e));
+          const float2 cs = angle(a, at.token, at.in_seq, pair_of(a, e));
           const float o = mine[partner(a, e)] * r;
           v = v * cs.x + (is_first(a, e) ? -o : o) * cs.y;
         }
@@ -151,12 +160,13 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
   for (long base = block * kWaves; base < total; base += blocks * kWaves) {
     const long row = base + wave;
     const bool live = row < total;
+    const Row at = row_of(a, s, live ? row : 0);
     const T* dy = (const T*)s.dy + row * a.dim;
     if (live)
       for (int e = lane; e < a.dim; e += 64) mine[e] = (float)dy[e];
     __syncthreads();
     if (live) {
-      const T* x = row_of<T>(a, s, row);
+      const T* x = (const T*)s.x + at.offset;
       T* dx = (T*)s.y + row * a.dim;
       float dn[kMaxDim / 64];
       float sum = 0.f, dot = 0.f;
@@ -166,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
         if (e >= a.dim) continue;
         float v = mine[e];
         if (e < 2 * a.half) {
-          const float2 cs = angle(a, row / s.heads, pair_of(a, e));
+          const float2 cs = angle(a, at.token, at.in_seq, pair_of(a, e));
           const float o = mine[partner(a, e)];
           v = v * cs.x + (is_first(a, e) ? o : -o) * cs.y;
         }
@@ -200,7 +210,8 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
 // Rows in registers: G lanes hold a row, 8 values each, so a wave works on
 // 64 / G heads of one token at a time and goes through the token's heads of
 // queries, then keys.  The angles and positions of a token are read once.
-// Needs 16-byte rows: D, strides and pairs in multiples of 8 (see fits()).
+// Needs 16-byte rows: D and strides in multiples of 8, pairs in fours (see
+// fits()).
 //
 // Bound by memory.  Heads of more than elem::kCached are written past the
 // caches (NT): 16384 tokens of 32 + 8 heads of 128 in bf16 take 58 us forward
@@ -219,15 +230,22 @@ __device__ __forceinline__ void unpack(const Run<T>& w, float (&v)[kRun]) {
   for (int e = 0; e < kRun; ++e) v[e] = (float)w[e];
 }
 
-// The same run of another lane.
+// The halves of a run (4 values each) from two lanes; `crossed`: each as the
+// other half of those lanes' runs.
 template <typename T>
-__device__ __forceinline__ Run<T> from_lane(const Run<T>& w, int lane) {
-  constexpr int kWords = kRun * sizeof(T) / 4;
-  union { Run<T> run; int word[kWords]; } in, out;
+__device__ __forceinline__ Run<T> from_lanes(const Run<T>& w,
+                                             const int (&lane)[2],
+                                             bool crossed) {
+  constexpr int kHalf = kRun * sizeof(T) / 8;  // words
+  union { Run<T> run; int word[2 * kHalf]; } in, out;
   in.run = w;
   #pragma unroll
-  for (int i = 0; i < kWords; ++i)
-    out.word[i] = __builtin_amdgcn_ds_bpermute(lane << 2, in.word[i]);
+  for (int i = 0; i < 2 * kHalf; ++i) {
+    const int word = crossed ? in.word[(i + kHalf) % (2 * kHalf)]
+                             : in.word[i];
+    out.word[i] =
+        __builtin_amdgcn_ds_bpermute(lane[i / kHalf] << 2, word);
+  }
   return out.run;
 }
 
@@ -249,13 +267,15 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// What a lane keeps for all rows of a token: pairs are in the lane
-// (interleaved) or in the lane `other` (halves), `sign` is that of the
-// partner's term in the forward rotation.
+// What a lane keeps for all rows of a token.  Interleaved pairs are in the
+// lane: four from p0[0] on.  With halves the partners of each four values lie
+// in the lanes other[], in the other half of the run where pairs / 4 is odd
+// (crossed); they belong to four pairs from p0[] on, and sign[] is that of
+// the partner's term in the forward rotation.
 struct Lane {
-  int e0, other, p0;
-  bool on, turns;
-  float sign;
+  int e0, p0[2], other[2];
+  bool on, turns, crossed;
+  float sign[2];
 };
 
 template <int G, bool INTER>
@@ -265,21 +285,49 @@ __device__ __forceinline__ Lane lane_of(const Args& a) {
   l.e0 = sub * kRun;
   l.on = l.e0 < a.dim;
   l.turns = l.e0 < 2 * a.half;
-  l.other = lane;
-  l.sign = 1.f;
-  if (INTER) {
-    l.p0 = l.e0 / 2;
-  } else {
-    const bool first = l.e0 < a.half;
-    l.p0 = first ? l.e0 : l.e0 - a.half;
-    if (l.turns) l.other = first ? lane + a.half / kRun
-                                 : lane - a.half / kRun;
-    l.sign = first ? -1.f : 1.f;
+  l.crossed = !INTER && (a.half / 4) % 2;
+  #pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int e = l.e0 + 4 * t;
+    const bool first = e < a.half;
+    l.p0[t] = INTER ? l.e0 / 2 : first ? e : e - a.half;
+    l.sign[t] = first ? -1.f : 1.f;
+    const int partner = first ? e + a.half : e - a.half;
+    l.other[t] = l.turns ? lane - sub + partner / kRun : lane;
   }
   return l;
 }
 
-// Angles of a lane's pairs at a token (the identity where nothing turns).
+// Cosines and sines of the four pairs from p on.
+__device__ __forceinline__ void angles4(const Args& a, long token,
+                                        long in_seq, int p, float* c,
+                                        float* s) {
+  int axis = 0;
+  while (axis + 1 < a.axes && p >= a.ends[axis]) ++axis;
+  if (axis + 1 < a.axes && p + 4 > a.ends[axis]) {
+    // on more than one axis
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 cs = angle(a, token, in_seq, p + i);
+      c[i] = cs.x;
+      s[i] = cs.y;
+    }
+    return;
+  }
+  const long at = a.pos ? a.pos[axis * a.tokens + token] : in_seq;
+  if (at < 0 || at >= a.table) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = s[i] = __uint_as_float(0x7fc00000);
+    return;
+  }
+  const float4 cv = *(const float4*)(a.cosines + at * a.half + p);
+  const float4 sv = *(const float4*)(a.sines + at * a.half + p);
+  c[0] = cv.x, c[1] = cv.y, c[2] = cv.z, c[3] = cv.w;
+  s[0] = sv.x, s[1] = sv.y, s[2] = sv.z, s[3] = sv.w;
+}
+
+// Angles of a lane at a token (the identity where nothing turns).  With
+// halves the sines carry the sign of the partner's term.
 template <bool INTER>
 __device__ __forceinline__ void angles(const Args& a, const Lane& l,
                                        long token, long in_seq, float* c,
@@ -291,44 +339,32 @@ __device__ __forceinline__ void angles(const Args& a, const Lane& l,
     s[i] = 0.f;
   }
   if (!l.turns) return;
-  int axis = 0;
-  while (axis + 1 < a.axes && l.p0 >= a.ends[axis]) ++axis;
-  if (axis + 1 < a.axes && l.p0 + P > a.ends[axis]) {
-    // the lane's pairs lie on more than one axis
-    #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float2 cs = angle(a, token, l.p0 + i);
-      c[i] = cs.x;
-      s[i] = cs.y;
-    }
-    return;
-  }
-  const long at = a.pos ? a.pos[axis * a.tokens + token] : in_seq;
-  if (at < 0 || at >= a.table) {
-    #pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = s[i] = __uint_as_float(0x7fc00000);
-    return;
-  }
-  const float4* cr = (const float4*)(a.cosines + at * a.half + l.p0);
-  const float4* sr = (const float4*)(a.sines + at * a.half + l.p0);
   #pragma unroll
-  for (int i = 0; i < P / 4; ++i) {
-    const float4 cv = cr[i], sv = sr[i];
-    c[4 * i] = cv.x, c[4 * i + 1] = cv.y;
-    c[4 * i + 2] = cv.z, c[4 * i + 3] = cv.w;
-    s[4 * i] = sv.x, s[4 * i + 1] = sv.y;
-    s[4 * i + 2] = sv.z, s[4 * i + 3] = sv.w;
+  for (int t = 0; t < P / 4; ++t) {
+    angles4(a, token, in_seq, l.p0[t], c + 4 * t, s + 4 * t);
+    if (!INTER) {
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * t + i] *= l.sign[t];
+    }
   }
 }
 
-template <typename T>
+// N weights from e0 on, zeros for a lane behind the row.
+template <typename T, int N>
 __device__ __forceinline__ void weights(const Args& a, const Side& s, int e0,
-                                        bool on, float (&w)[kRun]) {
+                                        bool on, float* w) {
   #pragma unroll
-  for (int e = 0; e < kRun; ++e) w[e] = on ? 1.f : 0.f;
+  for (int e = 0; e < N; ++e) w[e] = on ? 1.f : 0.f;
   if (!on || !s.w) return;
-  if (a.w_fp32) unpack<float>(*(const Run<float>*)((const float*)s.w + e0), w);
-  else unpack<T>(*(const Run<T>*)((const T*)s.w + e0), w);
+  if (a.w_fp32) {
+    const auto v = *(const elem::vec<float, N>*)((const float*)s.w + e0);
+    #pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = v[e];
+  } else {
+    const auto v = *(const elem::vec<T, N>*)((const T*)s.w + e0);
+    #pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = (float)v[e];
+  }
 }
 
 // Work of a wave: the heads [h0, h1) of a token, queries before keys.
@@ -379,11 +415,10 @@ __device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
       }
     } else {
       float vo[kRun];
-      unpack(from_lane<T>(raw, l.other), vo);
+      unpack(from_lanes<T>(raw, l.other, l.crossed), vo);
       #pragma unroll
       for (int e = 0; e < kRun; ++e)
-        o[e] = v[e] * r * w[e] * c[e] +
-               l.sign * sn[e] * (vo[e] * r * wo[e]);
+        o[e] = v[e] * r * w[e] * c[e] + sn[e] * (vo[e] * r * wo[e]);
     }
     if (l.on) {
       Run<T> out;
@@ -402,12 +437,15 @@ __global__ __launch_bounds__(kThreads) void fwd_rows_kernel(Args a,
   const Lane l = lane_of<G, INTER>(a);
   const int hq = a.side[0].heads;
   float wq[kRun], wk[kRun], woq[kRun], wok[kRun];
-  weights<T>(a, a.side[0], l.e0, l.on, wq);
-  weights<T>(a, a.side[1], l.e0, l.on, wk);
+  weights<T, kRun>(a, a.side[0], l.e0, l.on, wq);
+  weights<T, kRun>(a, a.side[1], l.e0, l.on, wk);
   if (!INTER) {
-    const int eo = (l.other % G) * kRun;
-    weights<T>(a, a.side[0], eo, l.on, woq);
-    weights<T>(a, a.side[1], eo, l.on, wok);
+    #pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int e = (l.other[t] % G) * kRun + 4 * (l.crossed ? 1 - t : t);
+      weights<T, 4>(a, a.side[0], e, l.on, woq + 4 * t);
+      weights<T, 4>(a, a.side[1], e, l.on, wok + 4 * t);
+    }
   }
   const long items = a.tokens * chunks;
   for (long i = (long)blockIdx.x * kWaves + (threadIdx.x >> 6); i < items;
@@ -452,10 +490,10 @@ __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
       }
     } else {
       float dp[kRun];
-      unpack(from_lane<T>(rawd, l.other), dp);
+      unpack(from_lanes<T>(rawd, l.other, l.crossed), dp);
       #pragma unroll
       for (int e = 0; e < kRun; ++e)
-        dn[e] = d[e] * c[e] - l.sign * sn[e] * dp[e];
+        dn[e] = d[e] * c[e] - sn[e] * dp[e];
     }
     float sum = 0.f, dot = 0.f;
     #pragma unroll
@@ -486,7 +524,7 @@ __global__ __launch_bounds__(kThreads) void bwd_rows_kernel(
   float w[2][kRun], dw[2][kRun];
   #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    weights<T>(a, a.side[side], l.e0, l.on, w[side]);
+    weights<T, kRun>(a, a.side[side], l.e0, l.on, w[side]);
     #pragma unroll
     for (int e = 0; e < kRun; ++e) dw[side][e] = 0.f;
   }
@@ -642,7 +680,7 @@ void share(const Args& a, long most, int& q_blocks, int& blocks) {
 // Whether the kernels with rows in registers take the call.
 bool fits(const Args& a, size_t size) {
   if (a.dim % kRun || a.dim > 64 * kRun) return false;
-  if (a.half % (a.interleaved ? kRun / 2 : kRun)) return false;
+  if (a.half % 4) return false;
   if (!elem::aligned16(a.cosines) || !elem::aligned16(a.sines)) return false;
   for (const Side& s : a.side) {
     if (!elem::aligned16(s.x) || !elem::aligned16(s.dy) ||
@@ -914,6 +952,7 @@ std::vector<at::Tensor> qk_norm_rope(
        (t.wq.defined() && t.wq.requires_grad()) ||
        (t.wk.defined() && t.wk.requires_grad()));
   if (!grad) return forward_of(t, m);
+  elem::check_capture({q, k, t.wq, t.wk});
   // variables among the arguments are found as tensors of their own
   return QKNormRope::apply(
       t.q, t.k, wq ? std::optional<at::Tensor>(t.wq) : std::nullopt,

@@ -24,6 +24,7 @@ namespace {
 using elem::kVec;
 
 constexpr int kThreads = 256;
+constexpr float kLowest = -3.402823466e38f;  // finite
 
 struct Shape {
   long rows, vocab;        // rows = outer * inner
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(THREADS) void row_stats_kernel(
   const int body = (n - head) / V;
   const bool mine = threadIdx.x == 0 && t >= begin && t < begin + n;
   const float xt = mine ? (float)x[t - begin] : 0.f;
-  float m = -3.402823466e38f, sum = 0.f;
+  float m = kLowest, sum = 0.f;
   const Vec* xv = (const Vec*)(x + head);
   int i = threadIdx.x;
   for (; i + 3 * THREADS < body; i += 4 * THREADS) {
@@ -172,6 +173,7 @@ __device__ __forceinline__ RowLp row_lp(const float2* __restrict__ stats,
                                         const float* __restrict__ picked,
                                         long row, int pieces) {
   float2 a = stats[row * pieces];
+  #pragma unroll 8
   for (int p = 1; p < pieces; ++p) {
     const float2 b = stats[row * pieces + p];
     join(a.x, a.y, b.x, b.y);
@@ -185,21 +187,33 @@ __device__ __forceinline__ RowLp row_lp(const float2* __restrict__ stats,
 
 // What the backward needs of a row is saved as four floats: M, 1 / sum, lp
 // and the row's coefficient.
-__global__ __launch_bounds__(kThreads) void lp_finish_kernel(
+// A wave for each row, of which there are few and the pieces many.
+__global__ __launch_bounds__(64) void lp_finish_kernel(
     const long* __restrict__ target, const float2* __restrict__ stats,
     const float* __restrict__ picked, float4* __restrict__ saved,
     float* __restrict__ lp, Shape s, long ignore, int pieces) {
-  const long row = (long)blockIdx.x * kThreads + threadIdx.x;
-  if (row >= s.rows) return;
-  const long t = target[row];
-  if (!is_live(t, s.vocab, ignore)) {
-    lp[row] = 0.f;
-    if (saved) saved[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const long row = blockIdx.x;
+  const int lane = threadIdx.x;
+  if (!is_live(target[row], s.vocab, ignore)) {
+    if (lane == 0) {
+      lp[row] = 0.f;
+      if (saved) saved[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     return;
   }
-  const RowLp r = row_lp(stats, picked, row, pieces);
-  lp[row] = (float)r.lp;
-  if (saved) saved[row] = make_float4(r.m, r.inv, (float)r.lp, 1.f);
+  float m = kLowest, sum = 0.f;
+  for (int p = lane; p < pieces; p += 64) {
+    const float2 b = stats[row * pieces + p];
+    join(m, sum, b.x, b.y);
+  }
+  #pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    join(m, sum, __shfl_xor(m, off), __shfl_xor(sum, off));
+  if (lane == 0) {
+    const double l = (double)picked[row] - (double)m - log((double)sum);
+    lp[row] = (float)l;
+    if (saved) saved[row] = make_float4(m, 1.f / sum, (float)l, 1.f);
+  }
 }
 
 template <int THREADS>
@@ -507,7 +521,9 @@ at::Tensor per_token(const at::Tensor& v, const at::Tensor& target,
 }
 
 bool wants_grad(const at::Tensor& x) {
-  return at::GradMode::is_enabled() && x.requires_grad();
+  if (!at::GradMode::is_enabled() || !x.requires_grad()) return false;
+  elem::check_capture({x});
+  return true;
 }
 
 // Temporary memory of a forward call: the blocks' partial sums in fp64, the
@@ -588,6 +604,14 @@ at::Tensor saved_for(const at::Tensor& logits, long rows, long scales) {
   return at::empty({4 * rows + scales}, logits.options().dtype(at::kFloat));
 }
 
+// Calls of few rows whose rows one block of 1024 takes whole, which saves the
+// second launch: short rows (50257 bf16: 6.0 against 7.6 us, while one row of
+// 128256 is faster split, 7.3 against 9.9 us), and rows that fill half the
+// chip without a split (200 of 128256: 12.6 against 15.0 us).
+bool takes_whole_rows(long rows, long bytes) {
+  return bytes <= (160L << 10) || rows >= 128;
+}
+
 // (lp [...] fp32); saved may be undefined.
 at::Tensor logprobs_forward(const at::Tensor& logits,
                             const at::Tensor& target, long ignore,
@@ -598,19 +622,23 @@ at::Tensor logprobs_forward(const at::Tensor& logits,
   if (c.s.rows == 0) return lp;
   float4* keep = saved.defined() ? (float4*)saved.data_ptr() : nullptr;
   STOKE_ELEM_SWITCH(logits.scalar_type(), "token_logprobs", {
-    if (c.pieces == 1) {
-      hipLaunchKernelGGL((row_stats_kernel<T, kThreads, true>),
-                         dim3((unsigned)c.s.rows), dim3(kThreads), 0,
+    const auto whole_rows = [&](auto threads) {
+      hipLaunchKernelGGL((row_stats_kernel<T, threads, true>),
+                         dim3((unsigned)c.s.rows), dim3(threads), 0,
                          elem::stream(), (const T*)logits.data_ptr(),
                          target.data_ptr<long>(), nullptr, nullptr, nullptr,
-                         c.s, ignore, 1, c.piece, keep, lp.data_ptr<float>());
+                         c.s, ignore, 1, c.s.vocab, keep,
+                         lp.data_ptr<float>());
+    };
+    if (c.pieces == 1) {
+      whole_rows(std::integral_constant<int, kThreads>{});
+    } else if (takes_whole_rows(c.s.rows, c.s.vocab * (long)sizeof(T))) {
+      whole_rows(std::integral_constant<int, 1024>{});
     } else {
       const Scratch tmp(logits, 0, c);
       launch_stats<T>(logits, target, c, tmp);
       hipLaunchKernelGGL(
-          lp_finish_kernel,
-          dim3((unsigned)((c.s.rows + kThreads - 1) / kThreads)),
-          dim3(kThreads), 0, elem::stream(), target.data_ptr<long>(),
+          lp_finish_kernel, dim3((unsigned)c.s.rows), dim3(64), 0, elem::stream(), target.data_ptr<long>(),
           tmp.stats, tmp.picked, keep, lp.data_ptr<float>(),
           c.s, ignore, c.pieces);
     }

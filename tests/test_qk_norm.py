@@ -111,6 +111,9 @@ CASES = [
     (1, 17, 6, 3, 96, 96, 3),
     (2, 65, 5, 1, 128, 128, 3),
     (2, 9, 4, 4, 128, 64, 1),
+    (2, 11, 4, 2, 128, 24, 1),
+    (1, 6, 2, 2, 80, 72, 3),
+    (1, 9, 2, 1, 512, 8, 1),
     (1, 31, 2, 2, 192, 96, 4),
     (1, 40, 4, 1, 256, 256, 2),
     (1, 3, 2, 1, 600, 200, 1),
@@ -359,3 +362,21 @@ def test_gpu_repeats_and_replays_bit_for_bit():
         torch.cuda.synchronize()
         got = [v.clone() for v in out]
         assert all(torch.equal(a, b) for a, b in zip(got, step())), i
+
+
+@pytest.mark.gpu
+def test_gpu_capture_over_a_live_graph_of_the_weights_is_refused():
+    _skip("cuda")
+    (q, k, qw, kw, cos, sin, pos, dq, dk), _ = _case(
+        2, 6, 3, 1, 64, 64, torch.bfloat16, torch.float32, device="cuda")
+    kw.requires_grad_(True)
+    alive = qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="drop that graph"):
+            qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos)
+        with torch.no_grad():
+            out = qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos)
+    graph.replay()
+    assert torch.equal(out[0], alive[0]) and torch.equal(out[1], alive[1])

@@ -464,3 +464,50 @@ def test_gpu_second_derivative_is_refused():
         g, = torch.autograd.grad(loss, x, create_graph=True)
         with pytest.raises(RuntimeError):
             g.square().sum().backward()
+
+
+@pytest.mark.gpu
+def test_gpu_logits_of_more_than_2_31_elements():
+    _skip("cuda")
+    rows, v = 18000, 128256
+    x = torch.empty(1, rows, v, dtype=torch.bfloat16, device="cuda")
+    x[0, 0].normal_(generator=torch.Generator("cuda").manual_seed(0))
+    x[:, 1:] = 0
+    x[0, -1] = x[0, 0]
+    x.requires_grad_(True)
+    t = torch.full((1, rows), IGN, device="cuda")
+    t[0, 0] = t[0, -1] = 77
+    t[0, 17000] = 5
+    lp = token_logprobs(x, t)
+    # equal rows at both ends, a uniform row past 2^31 elements
+    assert float(lp[0, 0].detach()) == float(lp[0, -1].detach())
+    assert abs(float(lp[0, 17000].detach()) + 11.761783) < 1e-5
+    lp.sum().backward()
+    assert torch.equal(x.grad[0, 0], x.grad[0, -1])
+    assert abs(float(x.grad[0, 17000].float().sum())) < 1e-2
+    assert bool((x.grad[0, 17000] != 0).all())
+    assert bool((x.grad[0, 1:17000:997] == 0).all())
+
+
+@pytest.mark.gpu
+def test_gpu_capture_over_a_live_graph_of_the_same_leaf_is_refused():
+    _skip("cuda")
+    x, t = _inputs((2, 3, 50), torch.float32, "cuda", keep=1.0)
+    x.requires_grad_(True)
+    alive = token_logprobs(x, t)  # a graph of the default stream
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="drop that graph"):
+            token_logprobs(x, t)
+        with torch.no_grad():
+            out = token_logprobs(x, t)
+    graph.replay()
+    assert torch.equal(out, alive.detach())
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, = torch.autograd.grad(token_logprobs(x, t).sum(), x)
+    graph.replay()
+    want, = torch.autograd.grad(token_logprobs(x, t).sum(), x)
+    assert torch.equal(out, want)
