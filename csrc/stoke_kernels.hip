@@ -691,8 +691,9 @@ std::vector<at::Tensor> fp8_quant_t(at::Tensor x, at::Tensor scale,
                                     at::Tensor amax_next, int64_t kind);
 
 // Activations held in 8 bits (csrc/act8.hip)
-std::vector<at::Tensor> act8_pack(at::Tensor x);
-at::Tensor act8_unpack(at::Tensor q, at::Tensor scale, at::ScalarType dtype);
+std::vector<at::Tensor> act8_pack(at::Tensor act);
+at::Tensor act8_unpack(at::Tensor values, at::Tensor scales,
+                       at::ScalarType dtype);
 at::Tensor swiglu8(at::Tensor g, at::Tensor u);
 
 // Token log-probabilities and the losses on them (csrc/token_loss.hip)

@@ -71,31 +71,29 @@ def _eager_unpack(q: torch.Tensor, scale: torch.Tensor,
 
 def compress_activation(x: torch.Tensor) -> CompressedActivation:
     """``x`` (bf16, fp16 or fp32, any shape) in 8 bits, without gradient."""
+    if x.is_cuda:
+        # the extension checks its arguments in the same way
+        return CompressedActivation(*ops._require_ext().act8_pack(x), x.dtype)
     if x.dtype not in _DTYPES:
         raise ValueError(
             f"Stoke -- compress_activation takes bf16, fp16 or fp32, got "
             f"{x.dtype}"
         )
-    if x.is_cuda:
-        q, scale = ops._require_ext().act8_pack(x.detach().contiguous())
-    else:
-        q, scale = _eager_pack(x)
-    return CompressedActivation(q, scale, x.dtype)
+    return CompressedActivation(*_eager_pack(x), x.dtype)
 
 
 def restore_activation(held: CompressedActivation) -> torch.Tensor:
     """The values that ``held`` stands for, in the activation's dtype."""
     q, scale, dtype = held
+    if q.is_cuda:
+        return ops._require_ext().act8_unpack(q, scale, dtype)
     if dtype not in _DTYPES or q.dtype != torch.int8 \
-            or scale.dtype != torch.uint8 \
+            or scale.dtype != torch.uint8 or scale.is_cuda \
             or scale.numel() != (q.numel() + _BLOCK - 1) // _BLOCK:
         raise ValueError(
             "Stoke -- restore_activation takes what compress_activation "
             "returned: int8 values and one uint8 exponent for every 32"
         )
-    if q.is_cuda:
-        return ops._require_ext().act8_unpack(q.contiguous(),
-                                              scale.contiguous(), dtype)
     return _eager_unpack(q, scale, dtype)
 
 

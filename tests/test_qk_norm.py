@@ -64,8 +64,9 @@ def _oracle(x, w, dy, cos, sin, pos, sections, eps, inter):
     def turn(v, sn, absolute=False):
         out = v.clone().abs() if absolute else v.clone()
         if absolute:
-            out[..., a] = v[..., a].abs() * c.abs() + v[..., b].abs() * sn.abs()
-            out[..., b] = v[..., b].abs() * c.abs() + v[..., a].abs() * sn.abs()
+            v, ca, sa = v.abs(), c.abs(), sn.abs()
+            out[..., a] = v[..., a] * ca + v[..., b] * sa
+            out[..., b] = v[..., b] * ca + v[..., a] * sa
         else:
             out[..., a] = v[..., a] * c - v[..., b] * sn
             out[..., b] = v[..., b] * c + v[..., a] * sn
