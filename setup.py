@@ -27,6 +27,7 @@ setup(
         "stoke.shard",
         "stoke.amp",
         "stoke.ops",
+        "stoke.nn",
     ],
     ext_modules=[
         cpp_extension.CUDAExtension(
