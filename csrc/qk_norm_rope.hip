@@ -910,6 +910,13 @@ void check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq,
                     "device, got ", pos->sizes(), " ", pos->scalar_type());
 }
 
+// Weights may lie anywhere in a flat parameter: D values are copied sooner
+// than every row goes the slow way.
+at::Tensor aligned(const at::Tensor& w) {
+  const at::Tensor x = w.contiguous();
+  return elem::aligned16(x.data_ptr()) ? x : x.clone();
+}
+
 at::Tensor unit_stride(const at::Tensor& x) {
   return x.size(3) > 1 && x.stride(3) != 1 ? x.contiguous() : x;
 }
@@ -930,8 +937,8 @@ std::vector<at::Tensor> qk_norm_rope(
     std::optional<std::vector<int64_t>> sections, double eps,
     bool interleaved) {
   Tensors t;
-  if (wq) t.wq = wq->contiguous();
-  if (wk) t.wk = wk->contiguous();
+  if (wq) t.wq = aligned(*wq);
+  if (wk) t.wk = aligned(*wk);
   check(q, k, t.wq, t.wk, cosines, sines, pos, sections);
   t.q = unit_stride(q);
   t.k = unit_stride(k);
@@ -952,7 +959,8 @@ std::vector<at::Tensor> qk_norm_rope(
        (t.wq.defined() && t.wq.requires_grad()) ||
        (t.wk.defined() && t.wk.requires_grad()));
   if (!grad) return forward_of(t, m);
-  elem::check_capture({q, k, t.wq, t.wk});
+  elem::check_capture({q, k, wq.value_or(at::Tensor()),
+                       wk.value_or(at::Tensor())});
   // variables among the arguments are found as tensors of their own
   return QKNormRope::apply(
       t.q, t.k, wq ? std::optional<at::Tensor>(t.wq) : std::nullopt,

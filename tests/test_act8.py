@@ -395,3 +395,64 @@ def test_gpu_checkpoint8_saves_memory_under_autocast():
     per = 8192 * d
     assert held[16] >= (n + 1) * 2 * per
     assert held[8] <= n * per * 33 / 32 + 2 * per + (1 << 22)
+
+
+@pytest.mark.gpu
+def test_gpu_replays_in_a_graph():
+    _skip("cuda")
+    x = _act((64, 1000), torch.bfloat16, "cuda", 1)
+    u = _act((64, 1000), torch.bfloat16, "cuda", 2)
+    dy = _act((64, 1000), torch.bfloat16, "cuda", 3)
+    g = x.clone().requires_grad_(True)
+    u.requires_grad_(True)
+
+    def step():
+        held = compress_activation(g)
+        y = swiglu(g, u, save_bits=8)
+        return (held.values, held.scales, restore_activation(held),
+                y.detach(), *torch.autograd.grad(y, (g, u), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            g.copy_(x * (1 + 3 * i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), i
+
+
+@pytest.mark.gpu
+def test_gpu_tensors_past_the_cached_size():
+    """Large tensors take other accesses: the same values."""
+    _skip("cuda")
+    n = (65 << 20) + 40  # bf16: over 128 MB, an odd last block
+    x = torch.randn(n, device="cuda", dtype=torch.bfloat16,
+                    generator=torch.Generator("cuda").manual_seed(0))
+    held = compress_activation(x)
+    back = restore_activation(held)
+    dy = x.flip(0)
+    u = dy.clone()
+    g, u = x.clone().requires_grad_(True), u.requires_grad_(True)
+    y = swiglu(g, u, save_bits=8)
+    dg, du = torch.autograd.grad(y, (g, u), dy)
+    step = 32 << 20
+    for a in range(0, n, step):
+        b = min(n, a + step)
+        part = compress_activation(x[a:b])
+        assert torch.equal(part.values, held.values[a:b])
+        assert torch.equal(part.scales, held.scales[a // 32:(b + 31) // 32])
+        assert torch.equal(restore_activation(part), back[a:b])
+        gp = x[a:b].clone().requires_grad_(True)
+        up = u.detach()[a:b].clone().requires_grad_(True)
+        yp = swiglu(gp, up, save_bits=8)
+        assert torch.equal(yp, y[a:b])
+        dgp, dup = torch.autograd.grad(yp, (gp, up), dy[a:b])
+        assert torch.equal(dgp, dg[a:b]) and torch.equal(dup, du[a:b])

@@ -201,6 +201,19 @@ def test_matches_the_norm_and_rope_it_replaces(device):
     for p in (at, at[:1], at.int()):
         zq, zk = mod(q, k, cos, sin, positions=p)
         assert torch.equal(zq, yq) and torch.equal(zk, yk)
+    # weights that lie anywhere in a flat parameter
+    flat = torch.cat((qw[:3], qw, kw)).requires_grad_(True)
+    zq, zk = qk_norm_rope(q, k, flat[3:67], flat[67:], cos, sin)
+    assert torch.equal(zq, yq) and torch.equal(zk, yk)
+    gf, = torch.autograd.grad((zq, zk), flat, (dq, dk))
+    gw = torch.autograd.grad((yq, yk), (mod.q_weight, mod.k_weight), (dq, dk))
+    assert torch.equal(gf[3:67], gw[0]) and torch.equal(gf[67:], gw[1])
+    # positions of several axes broadcast over the batch
+    p3 = torch.stack((at[0], at[0].flip(0)))[:, None]
+    za = mod(q, k, cos, sin, positions=p3, sections=[20, 12])
+    zb = mod(q, k, cos, sin, positions=p3.expand(2, 2, 12).contiguous(),
+             sections=(20, 12))
+    assert torch.equal(za[0], zb[0]) and torch.equal(za[1], zb[1])
     # one section for all pairs is the single axis
     zq, _ = mod(q, k, cos, sin, positions=at[None], sections=[32])
     assert torch.equal(zq, yq)
@@ -381,3 +394,41 @@ def test_gpu_capture_over_a_live_graph_of_the_weights_is_refused():
             out = qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos)
     graph.replay()
     assert torch.equal(out[0], alive[0]) and torch.equal(out[1], alive[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inter", [True, False])
+def test_gpu_heads_past_the_cached_size(inter):
+    """Large calls take other accesses: the same values."""
+    _skip("cuda")
+    b, s, hq, hk, d = 4, 4097, 32, 8, 128
+    (q, k, qw, kw, cos, sin, pos, dq, dk), sec = _case(
+        b, 1, hq, hk, d, d, torch.bfloat16, torch.float32, axes=3,
+        device="cuda")
+    gen = torch.Generator("cuda").manual_seed(0)
+    q, k, dq, dk = (torch.randn(b, s, h, d, device="cuda", generator=gen,
+                                dtype=torch.bfloat16)
+                    for h in (hq, hk, hq, hk))
+    pos = torch.randint(0, 300, (3, b, s), device="cuda", generator=gen)
+    for w in (q, k, qw, kw):
+        w.requires_grad_(True)
+    y = qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos, sections=sec,
+                     interleaved=inter)
+    g = torch.autograd.grad(y, (q, k, qw, kw), (dq, dk))
+    dw = [torch.zeros(d, dtype=torch.float64, device="cuda")] * 2
+    for i in range(b):
+        x = [v.detach()[i:i + 1].requires_grad_(True) for v in (q, k)]
+        yi = qk_norm_rope(*x, qw, kw, cos, sin, positions=pos[:, i:i + 1],
+                          sections=sec, interleaved=inter)
+        gi = torch.autograd.grad(yi, (*x, qw, kw),
+                                 (dq[i:i + 1], dk[i:i + 1]))
+        for whole, part in zip((*y, *g[:2]), (*yi, *gi[:2])):
+            assert torch.equal(whole[i:i + 1], part)
+        dw = [a + p.double() for a, p in zip(dw, gi[2:])]
+    for a, p, x, dy in zip(g[2:], dw, (q, k), (dq, dk)):
+        # both are sums of the same terms in another order: a wave adds up to
+        # 64 rows by itself, the rest is fp64; terms are |dn x r| with
+        # |dn| <= sqrt 2 max|dy| and |x r| <= |x| / rms
+        size = (2 ** 0.5 * dy.float().abs() * x.detach().float().abs()).sum(
+            (0, 1, 2)) * 2
+        assert bool(((a.double() - p).abs() <= 64 * U * size + 1e-6).all())

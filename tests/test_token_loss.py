@@ -511,3 +511,55 @@ def test_gpu_capture_over_a_live_graph_of_the_same_leaf_is_refused():
     graph.replay()
     want, = torch.autograd.grad(token_logprobs(x, t).sum(), x)
     assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [50257, 131072])
+def test_gpu_logits_past_the_cached_size(v):
+    """Large calls take other accesses and blocks: the same values."""
+    _skip("cuda")
+    b, s = 2, (140 << 20) // (4 * v) + 1  # bf16: over 128 MB
+    gen = torch.Generator("cuda").manual_seed(0)
+    x = torch.randn(b, s, v, device="cuda", dtype=torch.bfloat16,
+                    generator=gen)
+    t = torch.randint(0, v, (b, s), device="cuda", generator=gen)
+    t[:, ::3] = IGN
+    up = torch.randn(b, s, device="cuda", generator=gen)
+    x.requires_grad_(True)
+    lp = token_logprobs(x, t)
+    g, = torch.autograd.grad(lp, x, up)
+    for i in (0, 1, s // 2, s - 1):
+        o = Oracle(x[:, i:i + 1], t[:, i:i + 1])
+        off = (lp[:, i:i + 1].detach().cpu().double() - o.lp).abs()
+        assert bool((off <= o.tol_lp + U * o.lp.abs()).all())
+        c = up[:, i:i + 1].cpu().double()
+        o.grad(c, torch.zeros_like(c), torch.bfloat16, g[:, i:i + 1])
+
+
+@pytest.mark.gpu
+def test_gpu_two_streams_at_once():
+    _skip("cuda")
+    sets = []
+    for seed in (0, 1):
+        x, t = _inputs((4, 90, 3000), torch.bfloat16, "cuda", seed, keep=1.0)
+        o, old, adv, ref = _policy_inputs(x, t, seed)
+        sets.append([v.cuda() for v in (x, t, old, adv, ref)])
+
+    def step(x, t, old, adv, ref):
+        y = x.clone().requires_grad_(True)
+        a = fused_policy_loss(y, t, old, adv, ref, kl_coef=0.1)
+        b, r = fused_preference_loss(y, t, ref)
+        return (a.detach(), b.detach(), r,
+                *torch.autograd.grad((a, b), y))
+
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(step(*s))
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            assert all(torch.equal(p, q) for p, q in zip(w, g))
