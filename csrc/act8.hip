@@ -4,8 +4,9 @@
 // E and 32 signed bytes q with  value = q * 2^(E - 127),  |q| <= 127.
 // E is the least exponent from 1 up at which the block's largest value still
 // rounds into 127, so a value is off by at most half of 2^(E-127), that is
-// 1/127 of the block's largest.  Scaling by a power of two is exact: the one
-// rounding is the conversion to a whole number (half to even).  E = 255
+// 1/127 of the block's largest (2^-127 where that is below 2^-120 and E stays
+// at 1).  Scaling by a power of two is exact: the one rounding is the
+// conversion to a whole number (half to even).  E = 255
 // marks a block with an infinity or NaN; all of it reads back as NaN, so an
 // overflow in the forward pass still reaches the gradients.
 
