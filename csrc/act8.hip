@@ -108,7 +108,7 @@ __device__ __forceinline__ void unpack_run(const Bytes q, unsigned exp,
 template <bool NT, typename T>
 __device__ __forceinline__ void load_run(const T* __restrict__ p, long i,
                                          float (&v)[kRun]) {
-  const Run<T> w = elem::load<NT>((const Run<T>*)(p + i));
+  const Run<T> w = elem::load<NT, kRun>(p + i);
   #pragma unroll
   for (int e = 0; e < kRun; ++e) v[e] = (float)w[e];
 }
@@ -119,7 +119,7 @@ __device__ __forceinline__ void store_run(T* __restrict__ p, long i,
   Run<T> w;
   #pragma unroll
   for (int e = 0; e < kRun; ++e) w[e] = (T)v[e];
-  elem::store<NT>((Run<T>*)(p + i), w);
+  elem::store<NT, kRun>(p + i, w);
 }
 
 __device__ __forceinline__ float sigmoid(float a) {
@@ -139,10 +139,9 @@ __device__ __forceinline__ void swiglu_grad(float d, float a, float b,
   db = d * a * s;
 }
 
-// Every kernel has two forms.  The first takes 8 values a thread, with
-// 16-byte (or two 16-byte) accesses, for the whole blocks of 32; the last,
-// partial block and tensors that do not start on 16 bytes go one value a
-// thread.  `first` is where the second form begins, a multiple of 32.
+// Every kernel takes 8 values a thread, with 16-byte (or two 16-byte)
+// accesses, for the whole blocks of 32, and one value a thread for the last,
+// partial block, which begins at `first`.
 // NT: tensors over elem::kCached are read past the caches (and, in the
 // backward, written).  What the forward writes is read by the next product:
 // it goes through them.
@@ -185,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(
   const long me = (long)blockIdx.x * kThreads + threadIdx.x;
   for (long i = me * kRun; i < first; i += step * kRun) {
     float v[kRun];
-    unpack_run<T>(elem::load<NT>((const Bytes*)(q + i)), scale[i >> 5], v);
+    unpack_run<T>(elem::load<NT, kRun>(q + i), scale[i >> 5], v);
     store_run<false>(x, i, v);
   }
   for (long i = first + me; i < n; i += step)
@@ -248,8 +247,8 @@ __global__ __launch_bounds__(kThreads) void swiglu8_bwd_kernel(
   for (long i = me * kRun; i < first; i += step * kRun) {
     float d[kRun], a[kRun], b[kRun], da[kRun], db[kRun];
     load_run<NT>(dy, i, d);
-    unpack_run<T>(elem::load<NT>((const Bytes*)(qg + i)), sg[i >> 5], a);
-    unpack_run<T>(elem::load<NT>((const Bytes*)(qu + i)), su[i >> 5], b);
+    unpack_run<T>(elem::load<NT, kRun>(qg + i), sg[i >> 5], a);
+    unpack_run<T>(elem::load<NT, kRun>(qu + i), su[i >> 5], b);
     #pragma unroll
     for (int e = 0; e < kRun; ++e)
       swiglu_grad(d[e], a[e], b[e], da[e], db[e]);
@@ -265,11 +264,8 @@ __global__ __launch_bounds__(kThreads) void swiglu8_bwd_kernel(
   }
 }
 
-// Where the form of one value a thread begins.
-template <typename... P>
-long first_of(long n, P... p) {
-  return (elem::aligned16(p) && ...) ? n / 32 * 32 : 0;
-}
+// Where the last, partial block begins.
+inline long first_of(long n) { return n / 32 * 32; }
 
 inline dim3 grid_for(long n, long first, int runs = 1) {
   const long threads = std::max(first / kRun / runs, n - first);
@@ -314,7 +310,7 @@ at::Tensor swiglu8_forward(const at::Tensor& g, const at::Tensor& u,
   if (n == 0) return y;
   const Held h(held.data_ptr(), n);
   STOKE_ELEM_SWITCH(g.scalar_type(), "swiglu8", {
-    const long first = first_of(n, g.data_ptr(), u.data_ptr());
+    const long first = first_of(n);
     with_caching(n * (long)sizeof(T), [&](auto nt) {
       hipLaunchKernelGGL((swiglu8_fwd_kernel<T, nt>), grid_for(n, first),
                          dim3(kThreads), 0, elem::stream(),
@@ -333,7 +329,7 @@ variable_list swiglu8_backward(const at::Tensor& dy, const at::Tensor& held) {
   if (n == 0) return {dg, du};
   const Held h(held.data_ptr(), n);
   STOKE_ELEM_SWITCH(dy.scalar_type(), "swiglu8", {
-    const long first = first_of(n, dy.data_ptr());
+    const long first = first_of(n);
     with_caching(n * (long)sizeof(T), [&](auto nt) {
       hipLaunchKernelGGL((swiglu8_bwd_kernel<T, nt>), grid_for(n, first),
                          dim3(kThreads), 0, elem::stream(),
@@ -375,7 +371,7 @@ std::vector<at::Tensor> act8_pack(at::Tensor act) {
   auto q = at::empty(x.sizes(), x.options().dtype(at::kChar));
   auto scale = at::empty({(n + 31) / 32}, x.options().dtype(at::kByte));
   STOKE_ELEM_SWITCH(x.scalar_type(), "act8_pack", {
-    const long first = first_of(n, x.data_ptr());
+    const long first = first_of(n);
     // past the caches a thread takes two runs: 134M values 63 against 67 us
     if (n > 0)
       with_caching(n * (long)sizeof(T), [&](auto nt) {
@@ -405,7 +401,7 @@ at::Tensor act8_unpack(at::Tensor values, at::Tensor scales,
   const at::Tensor q = values.contiguous(), scale = scales.contiguous();
   auto x = at::empty(q.sizes(), q.options().dtype(dtype));
   STOKE_ELEM_SWITCH(dtype, "act8_unpack", {
-    const long first = first_of(n, q.data_ptr());
+    const long first = first_of(n);
     if (n > 0)
       with_caching(n * (long)sizeof(T), [&](auto nt) {
         hipLaunchKernelGGL((unpack_kernel<T, nt>),

@@ -20,19 +20,25 @@ using vec = T __attribute__((ext_vector_type(N)));
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// Vector accesses, past the caches where NT is set.
-template <bool NT, typename V>
-__device__ __forceinline__ V load(const V* p) {
-  using Words = vec<int, sizeof(V) / 4>;
-  if (!NT) return *p;
-  return __builtin_bit_cast(V, __builtin_nontemporal_load((const Words*)p));
+// N elements from any element on, past the caches where NT is set: one access
+// of 4, 8 or 16 bytes (two of 16) also where it does not start on as many.
+// That costs little: 134M bf16 values at an odd offset pack in 68 us instead
+// of 63.
+template <bool NT, int N, typename T>
+__device__ __forceinline__ vec<T, N> load(const T* p) {
+  typedef int Words __attribute__((ext_vector_type(N * sizeof(T) / 4),
+                                   aligned(sizeof(T)), may_alias));
+  const Words* w = (const Words*)p;
+  if (!NT) return __builtin_bit_cast(vec<T, N>, *w);
+  return __builtin_bit_cast(vec<T, N>, __builtin_nontemporal_load(w));
 }
-template <bool NT, typename V>
-__device__ __forceinline__ void store(V* p, const V& v) {
-  using Words = vec<int, sizeof(V) / 4>;
-  if (!NT) *p = v;
-  else
-    __builtin_nontemporal_store(__builtin_bit_cast(Words, v), (Words*)p);
+template <bool NT, int N, typename T>
+__device__ __forceinline__ void store(T* p, const vec<T, N>& v) {
+  typedef int Words __attribute__((ext_vector_type(N * sizeof(T) / 4),
+                                   aligned(sizeof(T)), may_alias));
+  const Words w = __builtin_bit_cast(Words, v);
+  if (!NT) *(Words*)p = w;
+  else __builtin_nontemporal_store(w, (Words*)p);
 }
 
 // Tensors up to this size stay in the 256 MB last-level cache next to what is
@@ -41,10 +47,6 @@ constexpr long kCached = 128L << 20;
 
 inline hipStream_t stream() {
   return at::hip::getCurrentHIPStream().stream();
-}
-
-inline bool aligned16(const void* p) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
 // A leaf's gradient belongs to the stream on which a graph first reached it,

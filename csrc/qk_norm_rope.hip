@@ -26,10 +26,11 @@ constexpr int kMaxDim = 1024;
 // Queries or keys.
 struct Side {
   const void* x;
-  const void* dy;  // backward; contiguous
+  const void* dy;  // backward
   void* y;         // forward output or dx; contiguous [B, S, H, D]
   const void* w;   // null: ones
   long sb, ss, sh;  // strides of x in elements
+  long db, ds, dh;  // and of dy: attention hands back [B, H, S, D]
   int heads;
 };
 
@@ -71,7 +72,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // Where a row lies.
 struct Row {
-  long token, in_seq, offset;  // of x
+  long token, in_seq, x, dy;  // offsets of x and dy
 };
 
 __device__ __forceinline__ Row row_of(const Args& a, const Side& s,
@@ -80,7 +81,9 @@ __device__ __forceinline__ Row row_of(const Args& a, const Side& s,
   r.token = row / s.heads;
   const long no = r.token / a.seq;
   r.in_seq = r.token - no * a.seq;
-  r.offset = no * s.sb + r.in_seq * s.ss + (row - r.token * s.heads) * s.sh;
+  const long head = row - r.token * s.heads;
+  r.x = no * s.sb + r.in_seq * s.ss + head * s.sh;
+  r.dy = no * s.db + r.in_seq * s.ds + head * s.dh;
   return r;
 }
 
@@ -97,8 +100,8 @@ __device__ __forceinline__ bool is_first(const Args& a, int e) {
   return a.interleaved ? (e & 1) == 0 : e < a.half;
 }
 
-// A wave for each row, the row in shared memory: any dim, stride and
-// alignment.
+// A wave for each row, the row in shared memory: any dim and any number of
+// pairs.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void fwd_any_kernel(Args a,
                                                            int q_blocks) {
@@ -116,7 +119,7 @@ __global__ __launch_bounds__(kThreads) void fwd_any_kernel(Args a,
     const Row at = row_of(a, s, live ? row : 0);
     float r = 0.f;
     if (live) {
-      const T* x = (const T*)s.x + at.offset;
+      const T* x = (const T*)s.x + at.x;
       float sum = 0.f;
       for (int e = lane; e < a.dim; e += 64) {
         const float v = (float)x[e];
@@ -161,12 +164,12 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
     const long row = base + wave;
     const bool live = row < total;
     const Row at = row_of(a, s, live ? row : 0);
-    const T* dy = (const T*)s.dy + row * a.dim;
+    const T* dy = (const T*)s.dy + at.dy;
     if (live)
       for (int e = lane; e < a.dim; e += 64) mine[e] = (float)dy[e];
     __syncthreads();
     if (live) {
-      const T* x = (const T*)s.x + at.offset;
+      const T* x = (const T*)s.x + at.x;
       T* dx = (T*)s.y + row * a.dim;
       float dn[kMaxDim / 64];
       float sum = 0.f, dot = 0.f;
@@ -210,8 +213,7 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
 // Rows in registers: G lanes hold a row, 8 values each, so a wave works on
 // 64 / G heads of one token at a time and goes through the token's heads of
 // queries, then keys.  The angles and positions of a token are read once.
-// Needs 16-byte rows: D and strides in multiples of 8, pairs in fours (see
-// fits()).
+// Needs D in eights and pairs in fours (see fits()), but no alignment.
 //
 // Bound by memory.  Heads of more than elem::kCached are written past the
 // caches (NT): 16384 tokens of 32 + 8 heads of 128 in bf16 take 58 us forward
@@ -320,10 +322,13 @@ __device__ __forceinline__ void angles4(const Args& a, long token,
     for (int i = 0; i < 4; ++i) c[i] = s[i] = __uint_as_float(0x7fc00000);
     return;
   }
-  const float4 cv = *(const float4*)(a.cosines + at * a.half + p);
-  const float4 sv = *(const float4*)(a.sines + at * a.half + p);
-  c[0] = cv.x, c[1] = cv.y, c[2] = cv.z, c[3] = cv.w;
-  s[0] = sv.x, s[1] = sv.y, s[2] = sv.z, s[3] = sv.w;
+  const auto cv = elem::load<false, 4>(a.cosines + at * a.half + p);
+  const auto sv = elem::load<false, 4>(a.sines + at * a.half + p);
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c[i] = cv[i];
+    s[i] = sv[i];
+  }
 }
 
 // Angles of a lane at a token (the identity where nothing turns).  With
@@ -357,11 +362,11 @@ __device__ __forceinline__ void weights(const Args& a, const Side& s, int e0,
   for (int e = 0; e < N; ++e) w[e] = on ? 1.f : 0.f;
   if (!on || !s.w) return;
   if (a.w_fp32) {
-    const auto v = *(const elem::vec<float, N>*)((const float*)s.w + e0);
+    const auto v = elem::load<false, N>((const float*)s.w + e0);
     #pragma unroll
     for (int e = 0; e < N; ++e) w[e] = v[e];
   } else {
-    const auto v = *(const elem::vec<T, N>*)((const T*)s.w + e0);
+    const auto v = elem::load<false, N>((const T*)s.w + e0);
     #pragma unroll
     for (int e = 0; e < N; ++e) w[e] = (float)v[e];
   }
@@ -397,7 +402,7 @@ __device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
   const float inv_dim = 1.f / (float)a.dim;
   for (int h = h0 + group; h < h1; h += 64 / G) {
     Run<T> raw = (Run<T>)(T)0.f;
-    if (l.on) raw = *(const Run<T>*)(x + h * s.sh);
+    if (l.on) raw = elem::load<false, kRun>(x + h * s.sh);
     float v[kRun], o[kRun];
     unpack(raw, v);
     float sum = 0.f;
@@ -424,7 +429,7 @@ __device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
       Run<T> out;
       #pragma unroll
       for (int e = 0; e < kRun; ++e) out[e] = (T)o[e];
-      elem::store<NT>((Run<T>*)(y + (long)h * a.dim), out);
+      elem::store<NT, kRun>(y + (long)h * a.dim, out);
     }
   }
 }
@@ -469,15 +474,14 @@ __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
                                          const float* sn) {
   const int group = (threadIdx.x & 63) / G;
   const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss + l.e0;
-  const long row0 = it.token * s.heads * a.dim + l.e0;
-  const T* dy = (const T*)s.dy + row0;
-  T* dx = (T*)s.y + row0;
+  const T* dy = (const T*)s.dy + it.seq_no * s.db + it.in_seq * s.ds + l.e0;
+  T* dx = (T*)s.y + it.token * s.heads * a.dim + l.e0;
   const float inv_dim = 1.f / (float)a.dim;
   for (int h = h0 + group; h < h1; h += 64 / G) {
     Run<T> raw = (Run<T>)(T)0.f, rawd = raw;
     if (l.on) {
-      raw = *(const Run<T>*)(x + h * s.sh);
-      rawd = *(const Run<T>*)(dy + (long)h * a.dim);
+      raw = elem::load<false, kRun>(x + h * s.sh);
+      rawd = elem::load<false, kRun>(dy + h * s.dh);
     }
     float v[kRun], d[kRun], dn[kRun];
     unpack(raw, v);
@@ -510,7 +514,7 @@ __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
       out[e] = (T)(r * (dn[e] * w[e] - v[e] * k));
       dw[e] += dn[e] * v[e] * r;
     }
-    if (l.on) elem::store<NT>((Run<T>*)(dx + (long)h * a.dim), out);
+    if (l.on) elem::store<NT, kRun>(dx + (long)h * a.dim, out);
   }
 }
 
@@ -617,6 +621,7 @@ void fill_side(Side& s, const at::Tensor& x,
                const at::Tensor& w, at::Tensor& y) {
   s.x = x.data_ptr();
   s.dy = nullptr;
+  s.db = s.ds = s.dh = 0;
   s.y = y.data_ptr();
   s.w = w.defined() ? w.data_ptr() : nullptr;
   s.sb = x.stride(0);
@@ -678,18 +683,8 @@ void share(const Args& a, long most, int& q_blocks, int& blocks) {
 }
 
 // Whether the kernels with rows in registers take the call.
-bool fits(const Args& a, size_t size) {
-  if (a.dim % kRun || a.dim > 64 * kRun) return false;
-  if (a.half % 4) return false;
-  if (!elem::aligned16(a.cosines) || !elem::aligned16(a.sines)) return false;
-  for (const Side& s : a.side) {
-    if (!elem::aligned16(s.x) || !elem::aligned16(s.dy) ||
-        !elem::aligned16(s.w))
-      return false;
-    const long step = 16 / (long)size;
-    if (s.sb % step || s.ss % step || s.sh % step) return false;
-  }
-  return true;
+bool fits(const Args& a) {
+  return a.dim % kRun == 0 && a.dim <= 64 * kRun && a.half % 4 == 0;
 }
 
 // Heads of a wave: all of a token's where the tokens alone fill the chip,
@@ -724,6 +719,11 @@ void with_layout(const Args& a, size_t size, F f) {
   else layout(std::integral_constant<int, 64>{});
 }
 
+// Rows with a unit stride inside, whatever the strides between them.
+at::Tensor unit_stride(const at::Tensor& x) {
+  return x.size(3) > 1 && x.stride(3) != 1 ? x.contiguous() : x;
+}
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -734,7 +734,7 @@ variable_list forward_of(const Tensors& t, const Mode& m) {
   const Args a = make_args(t, m, yq, yk);
   if (a.tokens * (a.side[0].heads + a.side[1].heads) == 0) return {yq, yk};
   STOKE_ELEM_SWITCH(t.q.scalar_type(), "qk_norm_rope", {
-    if (fits(a, sizeof(T))) {
+    if (fits(a)) {
       with_layout(a, sizeof(T), [&](auto lanes, auto inter, auto nt) {
         int chunks, per;
         divide(a, lanes, chunks, per);
@@ -761,8 +761,14 @@ variable_list backward_of(const Tensors& t, const Mode& m,
   auto dq = at::empty(t.q.sizes(), t.q.options());
   auto dk = at::empty(t.k.sizes(), t.k.options());
   Args a = make_args(t, m, dq, dk);
-  a.side[0].dy = dyq.data_ptr();
-  a.side[1].dy = dyk.data_ptr();
+  for (const int i : {0, 1}) {
+    const at::Tensor& dy = i ? dyk : dyq;
+    Side& s = a.side[i];
+    s.dy = dy.data_ptr();
+    s.db = dy.stride(0);
+    s.ds = dy.stride(1);
+    s.dh = dy.stride(2);
+  }
   at::Tensor dwq, dwk;
   if (t.wq.defined()) dwq = at::empty(t.wq.sizes(), t.wq.options());
   if (t.wk.defined()) dwk = at::empty(t.wk.sizes(), t.wk.options());
@@ -776,7 +782,7 @@ variable_list backward_of(const Tensors& t, const Mode& m,
   const bool sums = dwq.defined() || dwk.defined();
   const auto f32 = t.q.options().dtype(at::kFloat);
   STOKE_ELEM_SWITCH(t.q.scalar_type(), "qk_norm_rope", {
-    if (fits(a, sizeof(T))) {
+    if (fits(a)) {
       with_layout(a, sizeof(T), [&](auto lanes, auto inter, auto nt) {
         int chunks, per;
         divide(a, lanes, chunks, per);
@@ -834,7 +840,7 @@ struct QKNormRope : torch::autograd::Function<QKNormRope> {
     const Mode m{ctx->saved_data["sections"].toIntVector(),
                  ctx->saved_data["eps"].toDouble(),
                  ctx->saved_data["interleaved"].toBool()};
-    const auto d = backward_of(t, m, dy[0].contiguous(), dy[1].contiguous());
+    const auto d = backward_of(t, m, unit_stride(dy[0]), unit_stride(dy[1]));
     variable_list out(6);
     std::copy(d.begin(), d.end(), out.begin());
     return elem::once_differentiable(std::move(out));
@@ -910,17 +916,6 @@ void check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq,
                     "device, got ", pos->sizes(), " ", pos->scalar_type());
 }
 
-// Weights may lie anywhere in a flat parameter: D values are copied sooner
-// than every row goes the slow way.
-at::Tensor aligned(const at::Tensor& w) {
-  const at::Tensor x = w.contiguous();
-  return elem::aligned16(x.data_ptr()) ? x : x.clone();
-}
-
-at::Tensor unit_stride(const at::Tensor& x) {
-  return x.size(3) > 1 && x.stride(3) != 1 ? x.contiguous() : x;
-}
-
 at::Tensor table32(const at::Tensor& x) {
   return x.scalar_type() == at::kFloat ? x.contiguous()
                                        : x.to(at::kFloat).contiguous();
@@ -937,8 +932,8 @@ std::vector<at::Tensor> qk_norm_rope(
     std::optional<std::vector<int64_t>> sections, double eps,
     bool interleaved) {
   Tensors t;
-  if (wq) t.wq = aligned(*wq);
-  if (wk) t.wk = aligned(*wk);
+  if (wq) t.wq = wq->contiguous();
+  if (wk) t.wk = wk->contiguous();
   check(q, k, t.wq, t.wk, cosines, sines, pos, sections);
   t.q = unit_stride(q);
   t.k = unit_stride(k);

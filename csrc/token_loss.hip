@@ -121,19 +121,20 @@ __global__ __launch_bounds__(THREADS) void row_stats_kernel(
   const bool mine = threadIdx.x == 0 && t >= begin && t < begin + n;
   const float xt = mine ? (float)x[t - begin] : 0.f;
   float m = kLowest, sum = 0.f;
-  const Vec* xv = (const Vec*)(x + head);
+  const T* xv = x + head;
   int i = threadIdx.x;
   for (; i + 3 * THREADS < body; i += 4 * THREADS) {
     Vec w[4];
     #pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = xv[i + u * THREADS];
+    for (int u = 0; u < 4; ++u)
+      w[u] = elem::load<false, V>(xv + (i + u * THREADS) * V);
     float v[4 * V];
     #pragma unroll
     for (int e = 0; e < 4 * V; ++e) v[e] = (float)w[e / V][e % V];
     take(v, m, sum);
   }
   for (; i < body; i += THREADS) {
-    const Vec w = xv[i];
+    const Vec w = elem::load<false, V>(xv + i * V);
     float v[V];
     #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = (float)w[e];
@@ -404,15 +405,16 @@ __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
   const int rest = n - body * V;
   const int lone = (int)threadIdx.x < head ? (int)threadIdx.x
                                            : (int)threadIdx.x + body * V;
-  Vec* dv = (Vec*)(dx + head);
+  T* dv = dx + head;
   if (c == 0.f) {
     const Vec zero = (Vec)(T)0.f;
     for (int i = threadIdx.x; i < body; i += THREADS)
-      elem::store<NT>(dv + i, zero);
+      elem::store<NT, V>(dv + i * V, zero);
     if ((int)threadIdx.x < rest) dx[lone] = (T)0.f;
     return;
   }
   const T* x = row_of(logits, s, row) + begin;
+  const T* xv = x + head;  // of another row stride: on other boundaries
   const float k = -c * r.y;
   // 1 - p of a token that is almost certain loses its digits
   const T at_target = (T)(-c * expm1f(r.z));
@@ -423,27 +425,20 @@ __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
     for (int e = 0; e < V; ++e) o[e] = (T)(k * exp_neg((float)w[e] - r.x));
     return o;
   };
-  if (head_of(x) == head_of(dx)) {
-    const Vec* xv = (const Vec*)(x + head);
-    int i = threadIdx.x;
-    for (; i + 3 * THREADS < body; i += 4 * THREADS) {
-      Vec w[4];
-      #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        w[u] = elem::load<NT>(xv + i + u * THREADS);
-      #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        elem::store<NT>(dv + i + u * THREADS, slope(w[u]));
-    }
-    for (; i < body; i += THREADS)
-      elem::store<NT>(dv + i, slope(elem::load<NT>(xv + i)));
-    if ((int)threadIdx.x < rest)
-      dx[lone] = (T)(k * exp_neg((float)x[lone] - r.x));
-  } else {
-    // logits of another row stride: their 16 bytes do not match the gradient's
-    for (int i = threadIdx.x; i < n; i += THREADS)
-      dx[i] = (T)(k * exp_neg((float)x[i] - r.x));
+  int i = threadIdx.x;
+  for (; i + 3 * THREADS < body; i += 4 * THREADS) {
+    Vec w[4];
+    #pragma unroll
+    for (int u = 0; u < 4; ++u)
+      w[u] = elem::load<NT, V>(xv + (i + u * THREADS) * V);
+    #pragma unroll
+    for (int u = 0; u < 4; ++u)
+      elem::store<NT, V>(dv + (i + u * THREADS) * V, slope(w[u]));
   }
+  for (; i < body; i += THREADS)
+    elem::store<NT, V>(dv + i * V, slope(elem::load<NT, V>(xv + i * V)));
+  if ((int)threadIdx.x < rest)
+    dx[lone] = (T)(k * exp_neg((float)x[lone] - r.x));
   __syncthreads();  // the target's own value last
   if (threadIdx.x == 0 && at >= 0 && at < n) dx[at] = at_target;
 }

@@ -182,6 +182,32 @@ def test_views_of_one_projection_and_other_layouts(d, inter, dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("d,inter", [(128, False), (64, True), (50, True)])
+def test_gradients_in_other_layouts(d, inter, device):
+    _skip(device)
+    (q, k, qw, kw, cos, sin, pos, dq, dk), _ = _case(
+        3, 7, 4, 2, d, d // 2 * 2, torch.bfloat16, torch.float32,
+        device=device)
+    leaves = [v.requires_grad_(True) for v in (q, k, qw, kw)]
+    y = qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos,
+                     interleaved=inter)
+
+    def run(a, b):
+        return torch.autograd.grad(y, leaves, (a, b), retain_graph=True)
+
+    want = run(dq, dk)
+    turn = [v.transpose(1, 2).contiguous().transpose(1, 2) for v in (dq, dk)]
+    last = [v.transpose(2, 3).contiguous().transpose(2, 3) for v in (dq, dk)]
+    for got in (run(*turn), run(dq, turn[1]), run(*last)):
+        assert all(torch.equal(p, r) for p, r in zip(got, want))
+    # one value for all: strides of 0
+    ones = [torch.ones((), dtype=v.dtype, device=device).expand(v.shape)
+            for v in (dq, dk)]
+    full = [v.contiguous() for v in ones]
+    assert all(torch.equal(p, r) for p, r in zip(run(*ones), run(*full)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_matches_the_norm_and_rope_it_replaces(device):
     _skip(device)
     (q, k, qw, kw, cos, sin, pos, dq, dk), _ = _case(
