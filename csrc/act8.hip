@@ -191,19 +191,37 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(
     x[i] = (T)restored<T>(q[i], scale[i >> 5]);
 }
 
+// Where the values of g and u lie: rows of `cols` values `g` and `u` elements
+// apart, as the halves of one projection are; contiguous where cols is 0.
+// Rows hold whole runs, and there are fewer than 2^31 values.
+struct Rows {
+  unsigned cols;
+  long g, u;
+};
+
 // y = silu(g) * u from the values as they come; g and u stay in 8 bits.
 template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     const T* __restrict__ g, const T* __restrict__ u, T* __restrict__ y,
     signed char* __restrict__ qg, signed char* __restrict__ qu,
     unsigned char* __restrict__ sg, unsigned char* __restrict__ su, long n,
-    long first) {
+    long first, Rows rows) {
   const long step = (long)gridDim.x * kThreads;
   const long me = (long)blockIdx.x * kThreads + threadIdx.x;
+  const auto place = [&](long i, long& ig, long& iu) {
+    ig = iu = i;
+    if (!rows.cols) return;
+    const unsigned row = (unsigned)i / rows.cols;
+    const long col = (unsigned)i - row * rows.cols;
+    ig = row * rows.g + col;
+    iu = row * rows.u + col;
+  };
   for (long i = me * kRun; i < first; i += step * kRun) {
     float a[kRun], b[kRun], o[kRun];
-    load_run<NT>(g, i, a);
-    load_run<NT>(u, i, b);
+    long ig, iu;
+    place(i, ig, iu);
+    load_run<NT>(g, ig, a);
+    load_run<NT>(u, iu, b);
     Bytes qa, qb;
     const unsigned ea = pack_run(a, qa), eb = pack_run(b, qb);
     #pragma unroll
@@ -218,8 +236,10 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
   }
   const long n32 = (n + 31) / 32 * 32;
   for (long i = first + me; i < n32; i += step) {
-    const float a = i < n ? (float)g[i] : 0.f;
-    const float b = i < n ? (float)u[i] : 0.f;
+    long ig, iu;
+    place(i, ig, iu);
+    const float a = i < n ? (float)g[ig] : 0.f;
+    const float b = i < n ? (float)u[iu] : 0.f;
     const unsigned eg =
         block_exponent(half_wave_max(__float_as_uint(a) & 0x7fffffff));
     const unsigned eu =
@@ -301,10 +321,33 @@ struct Held {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-at::Tensor swiglu8_forward(const at::Tensor& g, const at::Tensor& u,
+// The distance of x's rows where it is rows of contiguous values at one
+// positive distance from another, else 0.
+long row_step(const at::Tensor& x) {
+  const long d = x.dim();
+  if (d < 2 || x.stride(d - 1) != 1) return 0;
+  long step = 0, next = 0;
+  for (long i = d - 2; i >= 0; --i) {
+    if (x.size(i) == 1) continue;
+    if (x.stride(i) <= 0 || (step && x.stride(i) != next)) return 0;
+    if (!step) step = x.stride(i);
+    next = x.stride(i) * x.size(i);
+  }
+  return step;
+}
+
+at::Tensor swiglu8_forward(const at::Tensor& gate, const at::Tensor& up,
                            at::Tensor& held) {
-  const c10::DeviceGuard guard(g.device());
-  const long n = g.numel();
+  const c10::DeviceGuard guard(gate.device());
+  const long n = gate.numel();
+  Rows rows{0, 0, 0};
+  if (!gate.is_contiguous() || !up.is_contiguous()) {
+    rows = Rows{(unsigned)gate.size(-1), row_step(gate), row_step(up)};
+    if (n >= (1L << 31) || gate.size(-1) % kRun || !rows.g || !rows.u)
+      rows.cols = 0;
+  }
+  const at::Tensor g = rows.cols ? gate : gate.contiguous();
+  const at::Tensor u = rows.cols ? up : up.contiguous();
   auto y = at::empty(g.sizes(), g.options());
   held = at::empty({Held(nullptr, n).bytes}, g.options().dtype(at::kByte));
   if (n == 0) return y;
@@ -315,7 +358,8 @@ at::Tensor swiglu8_forward(const at::Tensor& g, const at::Tensor& u,
       hipLaunchKernelGGL((swiglu8_fwd_kernel<T, nt>), grid_for(n, first),
                          dim3(kThreads), 0, elem::stream(),
                          (const T*)g.data_ptr(), (const T*)u.data_ptr(),
-                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first);
+                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first,
+                         rows);
     });
   });
   return y;
@@ -344,7 +388,7 @@ struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& g,
                             const at::Tensor& u) {
     at::Tensor held;
-    auto y = swiglu8_forward(g.contiguous(), u.contiguous(), held);
+    auto y = swiglu8_forward(g, u, held);
     ctx->save_for_backward({held});
     return y;
   }

@@ -230,6 +230,35 @@ def test_swiglu8_strided_gradient_and_halves_of_one_projection(device):
     assert torch.equal(grad, torch.cat((dg, du), -1))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(6, 96), (1, 8), (5, 1, 40), (3, 7, 24),
+                                   (2, 3, 50), (4, 3), (9, 1), (300, 1000)])
+def test_swiglu8_rows_at_any_distance(shape, device):
+    _skip(device)
+    f = shape[-1]
+    wide = _act((*shape[:-1], 2 * f + 3), torch.bfloat16, device)
+    dense = _act(shape, torch.bfloat16, device, 4)
+    turned = dense.transpose(0, -1).contiguous().transpose(0, -1)
+    wider = _act((*shape[:-2], 2 * shape[-2], f), torch.bfloat16, device, 6)
+    pairs = [(wide[..., :f], wide[..., f:2 * f]),
+             (wide[..., 3:3 + f], dense), (dense, wide[..., -f:]),
+             (turned, dense), (dense, turned), (wider[..., ::2, :], dense),
+             (dense[..., :1].expand(shape), dense),
+             (dense[:1].expand(shape), dense),
+             (dense.narrow(-2, 0, 1).expand(shape), dense)]
+    for g, u in pairs:
+        g, u = g.detach().requires_grad_(True), u.detach().requires_grad_(True)
+        y = swiglu(g, u, save_bits=8)
+        got = torch.autograd.grad(y, (g, u), dense)
+        gc = g.detach().clone(memory_format=torch.contiguous_format)
+        uc = u.detach().clone(memory_format=torch.contiguous_format)
+        gc.requires_grad_(True), uc.requires_grad_(True)
+        yc = swiglu(gc, uc, save_bits=8)
+        want = torch.autograd.grad(yc, (gc, uc), dense)
+        assert torch.equal(y, yc)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # -------------------------------------------------------------- checkpoints
 class _Block(torch.nn.Module):
     def __init__(self, d):
