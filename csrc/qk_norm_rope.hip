@@ -223,34 +223,6 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
 // only lengthen the sum over blocks (4096: 10 us).
 constexpr int kRun = 8;
 
-template <typename T>
-using Run = elem::vec<T, kRun>;
-
-template <typename T>
-__device__ __forceinline__ void unpack(const Run<T>& w, float (&v)[kRun]) {
-  #pragma unroll
-  for (int e = 0; e < kRun; ++e) v[e] = (float)w[e];
-}
-
-// The halves of a run (4 values each) from two lanes; `crossed`: each as the
-// other half of those lanes' runs.
-template <typename T>
-__device__ __forceinline__ Run<T> from_lanes(const Run<T>& w,
-                                             const int (&lane)[2],
-                                             bool crossed) {
-  constexpr int kHalf = kRun * sizeof(T) / 8;  // words
-  union { Run<T> run; int word[2 * kHalf]; } in, out;
-  in.run = w;
-  #pragma unroll
-  for (int i = 0; i < 2 * kHalf; ++i) {
-    const int word = crossed ? in.word[(i + kHalf) % (2 * kHalf)]
-                             : in.word[i];
-    out.word[i] =
-        __builtin_amdgcn_ds_bpermute(lane[i / kHalf] << 2, word);
-  }
-  return out.run;
-}
-
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __int_as_float(
@@ -269,107 +241,188 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// What a lane keeps for all rows of a token.  Interleaved pairs are in the
-// lane: four from p0[0] on.  With halves the partners of each four values lie
-// in the lanes other[], in the other half of the run where pairs / 4 is odd
-// (crossed); they belong to four pairs from p0[] on, and sign[] is that of
-// the partner's term in the forward rotation.
+// What a lane holds of every row: four pairs from p on, or, behind the
+// rotated part, eight values that do not turn.  Interleaved pairs are the 8
+// values from `a` on; with halves the first values of the pairs are the 4
+// from `a` on and the second those from `b` on, so that no lane needs
+// another's values.
 struct Lane {
-  int e0, p0[2], other[2];
-  bool on, turns, crossed;
-  float sign[2];
+  int a, b, p;
+  bool on, turns;
 };
 
 template <int G, bool INTER>
-__device__ __forceinline__ Lane lane_of(const Args& a) {
-  const int lane = threadIdx.x & 63, sub = lane % G;
+__device__ __forceinline__ Lane lane_of(const Args& args) {
+  const int sub = threadIdx.x % G, turning = args.half / 4;
   Lane l;
-  l.e0 = sub * kRun;
-  l.on = l.e0 < a.dim;
-  l.turns = l.e0 < 2 * a.half;
-  l.crossed = !INTER && (a.half / 4) % 2;
-  #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int e = l.e0 + 4 * t;
-    const bool first = e < a.half;
-    l.p0[t] = INTER ? l.e0 / 2 : first ? e : e - a.half;
-    l.sign[t] = first ? -1.f : 1.f;
-    const int partner = first ? e + a.half : e - a.half;
-    l.other[t] = l.turns ? lane - sub + partner / kRun : lane;
+  l.turns = sub < turning;
+  l.p = 4 * sub;
+  l.a = kRun * sub;
+  l.b = l.a + 4;
+  if (!INTER && l.turns) {
+    l.a = l.p;
+    l.b = l.p + args.half;
   }
+  l.on = kRun * sub < args.dim;
   return l;
 }
 
-// Cosines and sines of the four pairs from p on.
-__device__ __forceinline__ void angles4(const Args& a, long token,
-                                        long in_seq, int p, float* c,
-                                        float* s) {
-  int axis = 0;
-  while (axis + 1 < a.axes && p >= a.ends[axis]) ++axis;
-  if (axis + 1 < a.axes && p + 4 > a.ends[axis]) {
-    // on more than one axis
+// The first and second values of a lane's pairs.
+struct Pairs {
+  float a[4], b[4];
+};
+
+template <typename T, bool INTER>
+__device__ __forceinline__ Pairs load(const Lane& l, const T* row) {
+  Pairs v;
+  if (INTER) {
+    const auto w = elem::load<false, kRun>(row + l.a);
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 cs = angle(a, token, in_seq, p + i);
-      c[i] = cs.x;
-      s[i] = cs.y;
+      v.a[i] = (float)w[2 * i];
+      v.b[i] = (float)w[2 * i + 1];
     }
-    return;
-  }
-  const long at = a.pos ? a.pos[axis * a.tokens + token] : in_seq;
-  if (at < 0 || at >= a.table) {
+  } else {
+    const auto wa = elem::load<false, 4>(row + l.a);
+    const auto wb = elem::load<false, 4>(row + l.b);
     #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = s[i] = __uint_as_float(0x7fc00000);
-    return;
+    for (int i = 0; i < 4; ++i) {
+      v.a[i] = (float)wa[i];
+      v.b[i] = (float)wb[i];
+    }
   }
-  const auto cv = elem::load<false, 4>(a.cosines + at * a.half + p);
-  const auto sv = elem::load<false, 4>(a.sines + at * a.half + p);
+  return v;
+}
+
+template <typename T, bool INTER, bool NT>
+__device__ __forceinline__ void store(const Lane& l, T* row, const Pairs& v) {
+  if (INTER) {
+    elem::vec<T, kRun> w;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[2 * i] = (T)v.a[i];
+      w[2 * i + 1] = (T)v.b[i];
+    }
+    elem::store<NT, kRun>(row + l.a, w);
+  } else {
+    elem::vec<T, 4> wa, wb;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      wa[i] = (T)v.a[i];
+      wb[i] = (T)v.b[i];
+    }
+    elem::store<NT, 4>(row + l.a, wa);
+    elem::store<NT, 4>(row + l.b, wb);
+  }
+}
+
+// Place of a lane's i-th pair in the row.
+template <bool INTER>
+__device__ __forceinline__ int first_at(const Lane& l, int i) {
+  return INTER ? l.a + 2 * i : l.a + i;
+}
+template <bool INTER>
+__device__ __forceinline__ int second_at(const Lane& l, int i) {
+  return INTER ? l.a + 2 * i + 1 : l.b + i;
+}
+
+// Where the rows of the tables that a token's axes take begin; negative
+// outside the tables.  The same for all lanes of a wave.
+struct Starts {
+  long at[kMaxAxes];
+};
+
+__device__ __forceinline__ Starts starts(const Args& a, long token,
+                                         long in_seq) {
+  Starts r;
+  #pragma unroll
+  for (int i = 0; i < kMaxAxes; ++i) {
+    r.at[i] = -1;
+    if (i >= a.axes) continue;
+    const long at = a.pos ? a.pos[i * a.tokens + token] : in_seq;
+    r.at[i] = at >= 0 && at < a.table ? at * a.half : -1;
+  }
+  return r;
+}
+
+// Sections of pairs follow each other.
+__device__ __forceinline__ int axis_of(const Args& a, int p) {
+  int axis = 0;
+  #pragma unroll
+  for (int i = 0; i + 1 < kMaxAxes; ++i)
+    axis += i + 1 < a.axes && p >= a.ends[i];
+  return axis;
+}
+
+// Chosen by the pair, not by the axis' number: an array indexed by a register
+// would be laid out in shared memory (72 instead of 58 us at the size above).
+__device__ __forceinline__ long start_of(const Args& a, const Starts& t,
+                                         int p) {
+  long at = t.at[0];
+  #pragma unroll
+  for (int i = 1; i < kMaxAxes; ++i)
+    if (i < a.axes && p >= a.ends[i - 1]) at = t.at[i];
+  return at;
+}
+
+// Cosines and sines of a lane's pairs; the identity where nothing turns.
+struct Angles {
+  float c[4], s[4];
+};
+
+__device__ __forceinline__ Angles angles(const Args& a, const Lane& l,
+                                         const Starts& t) {
+  const float nan = __uint_as_float(0x7fc00000);
+  Angles r;
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    c[i] = cv[i];
-    s[i] = sv[i];
+    r.c[i] = 1.f;
+    r.s[i] = 0.f;
   }
-}
-
-// Angles of a lane at a token (the identity where nothing turns).  With
-// halves the sines carry the sign of the partner's term.
-template <bool INTER>
-__device__ __forceinline__ void angles(const Args& a, const Lane& l,
-                                       long token, long in_seq, float* c,
-                                       float* s) {
-  constexpr int P = INTER ? kRun / 2 : kRun;
-  #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
-  }
-  if (!l.turns) return;
-  #pragma unroll
-  for (int t = 0; t < P / 4; ++t) {
-    angles4(a, token, in_seq, l.p0[t], c + 4 * t, s + 4 * t);
-    if (!INTER) {
+  if (!l.turns) return r;
+  if (axis_of(a, l.p) == axis_of(a, l.p + 3)) {
+    const long at = start_of(a, t, l.p);
+    if (at < 0) {
       #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * t + i] *= l.sign[t];
+      for (int i = 0; i < 4; ++i) r.c[i] = r.s[i] = nan;
+      return r;
     }
+    const auto c = elem::load<false, 4>(a.cosines + at + l.p);
+    const auto s = elem::load<false, 4>(a.sines + at + l.p);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.c[i] = c[i];
+      r.s[i] = s[i];
+    }
+    return r;
   }
+  // on more than one axis
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long from = start_of(a, t, l.p + i);
+    r.c[i] = from < 0 ? nan : a.cosines[from + l.p + i];
+    r.s[i] = from < 0 ? nan : a.sines[from + l.p + i];
+  }
+  return r;
 }
 
-// N weights from e0 on, zeros for a lane behind the row.
-template <typename T, int N>
-__device__ __forceinline__ void weights(const Args& a, const Side& s, int e0,
-                                        bool on, float* w) {
+// Weights of a lane's values, zeros for a lane behind the row.
+template <typename T, bool INTER>
+__device__ __forceinline__ Pairs weights(const Args& a, const Side& s,
+                                         const Lane& l) {
+  if (l.on && s.w)
+    return a.w_fp32 ? load<float, INTER>(l, (const float*)s.w)
+                    : load<T, INTER>(l, (const T*)s.w);
+  Pairs w;
   #pragma unroll
-  for (int e = 0; e < N; ++e) w[e] = on ? 1.f : 0.f;
-  if (!on || !s.w) return;
-  if (a.w_fp32) {
-    const auto v = elem::load<false, N>((const float*)s.w + e0);
-    #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = v[e];
-  } else {
-    const auto v = elem::load<false, N>((const T*)s.w + e0);
-    #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = (float)v[e];
-  }
+  for (int i = 0; i < 4; ++i) w.a[i] = w.b[i] = l.on ? 1.f : 0.f;
+  return w;
+}
+
+// The wave's number, known to be the same for its lanes: what follows from it
+// is computed and loaded once.
+__device__ __forceinline__ int wave_no() {
+  return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 }
 
 // Work of a wave: the heads [h0, h1) of a token, queries before keys.
@@ -392,45 +445,28 @@ __device__ __forceinline__ Item item_of(const Args& a, long item, int chunks,
 template <typename T, int G, bool INTER, bool NT>
 __device__ __forceinline__ void fwd_side(const Args& a, const Side& s,
                                          const Lane& l, const Item& it,
-                                         int h0, int h1,
-                                         const float (&w)[kRun],
-                                         const float (&wo)[kRun],
-                                         const float* c, const float* sn) {
+                                         int h0, int h1, const Pairs& w,
+                                         const Angles& t) {
   const int group = (threadIdx.x & 63) / G;
-  const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss + l.e0;
-  T* y = (T*)s.y + it.token * s.heads * a.dim + l.e0;
+  const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss;
+  T* y = (T*)s.y + it.token * s.heads * a.dim;
   const float inv_dim = 1.f / (float)a.dim;
   for (int h = h0 + group; h < h1; h += 64 / G) {
-    Run<T> raw = (Run<T>)(T)0.f;
-    if (l.on) raw = elem::load<false, kRun>(x + h * s.sh);
-    float v[kRun], o[kRun];
-    unpack(raw, v);
+    Pairs v = {};
+    if (l.on) v = load<T, INTER>(l, x + h * s.sh);
     float sum = 0.f;
     #pragma unroll
-    for (int e = 0; e < kRun; ++e) sum += v[e] * v[e];
+    for (int i = 0; i < 4; ++i) sum += v.a[i] * v.a[i] + v.b[i] * v.b[i];
     const float r =
         __builtin_amdgcn_rsqf(row_sum<G>(sum) * inv_dim + a.eps);
-    if (INTER) {
-      #pragma unroll
-      for (int i = 0; i < kRun / 2; ++i) {
-        const float p = v[2 * i] * r * w[2 * i];
-        const float q = v[2 * i + 1] * r * w[2 * i + 1];
-        o[2 * i] = p * c[i] - q * sn[i];
-        o[2 * i + 1] = q * c[i] + p * sn[i];
-      }
-    } else {
-      float vo[kRun];
-      unpack(from_lanes<T>(raw, l.other, l.crossed), vo);
-      #pragma unroll
-      for (int e = 0; e < kRun; ++e)
-        o[e] = v[e] * r * w[e] * c[e] + sn[e] * (vo[e] * r * wo[e]);
+    Pairs o;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = v.a[i] * r * w.a[i], q = v.b[i] * r * w.b[i];
+      o.a[i] = p * t.c[i] - q * t.s[i];
+      o.b[i] = q * t.c[i] + p * t.s[i];
     }
-    if (l.on) {
-      Run<T> out;
-      #pragma unroll
-      for (int e = 0; e < kRun; ++e) out[e] = (T)o[e];
-      elem::store<NT, kRun>(y + (long)h * a.dim, out);
-    }
+    if (l.on) store<T, INTER, NT>(l, y + (long)h * a.dim, o);
   }
 }
 
@@ -438,83 +474,58 @@ template <typename T, int G, bool INTER, bool NT>
 __global__ __launch_bounds__(kThreads) void fwd_rows_kernel(Args a,
                                                             int chunks,
                                                             int per) {
-  constexpr int P = INTER ? kRun / 2 : kRun;
   const Lane l = lane_of<G, INTER>(a);
   const int hq = a.side[0].heads;
-  float wq[kRun], wk[kRun], woq[kRun], wok[kRun];
-  weights<T, kRun>(a, a.side[0], l.e0, l.on, wq);
-  weights<T, kRun>(a, a.side[1], l.e0, l.on, wk);
-  if (!INTER) {
-    #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int e = (l.other[t] % G) * kRun + 4 * (l.crossed ? 1 - t : t);
-      weights<T, 4>(a, a.side[0], e, l.on, woq + 4 * t);
-      weights<T, 4>(a, a.side[1], e, l.on, wok + 4 * t);
-    }
-  }
+  const Pairs wq = weights<T, INTER>(a, a.side[0], l);
+  const Pairs wk = weights<T, INTER>(a, a.side[1], l);
   const long items = a.tokens * chunks;
-  for (long i = (long)blockIdx.x * kWaves + (threadIdx.x >> 6); i < items;
+  for (long i = (long)blockIdx.x * kWaves + wave_no(); i < items;
        i += (long)gridDim.x * kWaves) {
     const Item it = item_of(a, i, chunks, per);
-    float c[P], sn[P];
-    angles<INTER>(a, l, it.token, it.in_seq, c, sn);
+    const Angles t = angles(a, l, starts(a, it.token, it.in_seq));
     fwd_side<T, G, INTER, NT>(a, a.side[0], l, it, it.h0, min(it.h1, hq), wq,
-                          woq, c, sn);
+                              t);
     fwd_side<T, G, INTER, NT>(a, a.side[1], l, it, max(it.h0 - hq, 0),
-                          it.h1 - hq, wk, wok, c, sn);
+                              it.h1 - hq, wk, t);
   }
 }
 
 template <typename T, int G, bool INTER, bool NT>
 __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
                                          const Lane& l, const Item& it,
-                                         int h0, int h1,
-                                         const float (&w)[kRun],
-                                         float (&dw)[kRun], const float* c,
-                                         const float* sn) {
+                                         int h0, int h1, const Pairs& w,
+                                         Pairs& dw, const Angles& t) {
   const int group = (threadIdx.x & 63) / G;
-  const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss + l.e0;
-  const T* dy = (const T*)s.dy + it.seq_no * s.db + it.in_seq * s.ds + l.e0;
-  T* dx = (T*)s.y + it.token * s.heads * a.dim + l.e0;
+  const T* x = (const T*)s.x + it.seq_no * s.sb + it.in_seq * s.ss;
+  const T* dy = (const T*)s.dy + it.seq_no * s.db + it.in_seq * s.ds;
+  T* dx = (T*)s.y + it.token * s.heads * a.dim;
   const float inv_dim = 1.f / (float)a.dim;
   for (int h = h0 + group; h < h1; h += 64 / G) {
-    Run<T> raw = (Run<T>)(T)0.f, rawd = raw;
+    Pairs v = {}, d = {}, n;
     if (l.on) {
-      raw = elem::load<false, kRun>(x + h * s.sh);
-      rawd = elem::load<false, kRun>(dy + h * s.dh);
-    }
-    float v[kRun], d[kRun], dn[kRun];
-    unpack(raw, v);
-    unpack(rawd, d);
-    if (INTER) {
-      #pragma unroll
-      for (int i = 0; i < kRun / 2; ++i) {
-        dn[2 * i] = d[2 * i] * c[i] + d[2 * i + 1] * sn[i];
-        dn[2 * i + 1] = d[2 * i + 1] * c[i] - d[2 * i] * sn[i];
-      }
-    } else {
-      float dp[kRun];
-      unpack(from_lanes<T>(rawd, l.other, l.crossed), dp);
-      #pragma unroll
-      for (int e = 0; e < kRun; ++e)
-        dn[e] = d[e] * c[e] - sn[e] * dp[e];
+      v = load<T, INTER>(l, x + h * s.sh);
+      d = load<T, INTER>(l, dy + h * s.dh);
     }
     float sum = 0.f, dot = 0.f;
     #pragma unroll
-    for (int e = 0; e < kRun; ++e) {
-      sum += v[e] * v[e];
-      dot += dn[e] * w[e] * v[e];
+    for (int i = 0; i < 4; ++i) {
+      n.a[i] = d.a[i] * t.c[i] + d.b[i] * t.s[i];
+      n.b[i] = d.b[i] * t.c[i] - d.a[i] * t.s[i];
+      sum += v.a[i] * v.a[i] + v.b[i] * v.b[i];
+      dot += n.a[i] * w.a[i] * v.a[i] + n.b[i] * w.b[i] * v.b[i];
     }
     const float r =
         __builtin_amdgcn_rsqf(row_sum<G>(sum) * inv_dim + a.eps);
     const float k = row_sum<G>(dot) * inv_dim * r * r;
-    Run<T> out;
+    Pairs o;
     #pragma unroll
-    for (int e = 0; e < kRun; ++e) {
-      out[e] = (T)(r * (dn[e] * w[e] - v[e] * k));
-      dw[e] += dn[e] * v[e] * r;
+    for (int i = 0; i < 4; ++i) {
+      o.a[i] = r * (n.a[i] * w.a[i] - v.a[i] * k);
+      o.b[i] = r * (n.b[i] * w.b[i] - v.b[i] * k);
+      dw.a[i] += n.a[i] * v.a[i] * r;
+      dw.b[i] += n.b[i] * v.b[i] * r;
     }
-    if (l.on) elem::store<NT, kRun>(dx + (long)h * a.dim, out);
+    if (l.on) store<T, INTER, NT>(l, dx + (long)h * a.dim, o);
   }
 }
 
@@ -522,26 +533,20 @@ __device__ __forceinline__ void bwd_side(const Args& a, const Side& s,
 template <typename T, int G, bool INTER, bool NT>
 __global__ __launch_bounds__(kThreads) void bwd_rows_kernel(
     Args a, int chunks, int per, float* __restrict__ partial) {
-  constexpr int P = INTER ? kRun / 2 : kRun;
   const Lane l = lane_of<G, INTER>(a);
-  const int hq = a.side[0].heads, wave = threadIdx.x >> 6;
-  float w[2][kRun], dw[2][kRun];
-  #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    weights<T, kRun>(a, a.side[side], l.e0, l.on, w[side]);
-    #pragma unroll
-    for (int e = 0; e < kRun; ++e) dw[side][e] = 0.f;
-  }
+  const int hq = a.side[0].heads, wave = wave_no();
+  const Pairs wq = weights<T, INTER>(a, a.side[0], l);
+  const Pairs wk = weights<T, INTER>(a, a.side[1], l);
+  Pairs dw[2] = {};
   const long items = a.tokens * chunks;
   for (long i = (long)blockIdx.x * kWaves + wave; i < items;
        i += (long)gridDim.x * kWaves) {
     const Item it = item_of(a, i, chunks, per);
-    float c[P], sn[P];
-    angles<INTER>(a, l, it.token, it.in_seq, c, sn);
-    bwd_side<T, G, INTER, NT>(a, a.side[0], l, it, it.h0, min(it.h1, hq), w[0],
-                          dw[0], c, sn);
+    const Angles t = angles(a, l, starts(a, it.token, it.in_seq));
+    bwd_side<T, G, INTER, NT>(a, a.side[0], l, it, it.h0, min(it.h1, hq), wq,
+                              dw[0], t);
     bwd_side<T, G, INTER, NT>(a, a.side[1], l, it, max(it.h0 - hq, 0),
-                          it.h1 - hq, w[1], dw[1], c, sn);
+                              it.h1 - hq, wk, dw[1], t);
   }
   if (!partial) return;
   // over the wave's groups, then over the block's waves
@@ -549,11 +554,17 @@ __global__ __launch_bounds__(kThreads) void bwd_rows_kernel(
   #pragma unroll
   for (int side = 0; side < 2; ++side)
     #pragma unroll
-    for (int e = 0; e < kRun; ++e) {
-      float v = dw[side][e];
+    for (int i = 0; i < 4; ++i) {
+      float va = dw[side].a[i], vb = dw[side].b[i];
       #pragma unroll
-      for (int off = G; off < 64; off *= 2) v += __shfl_xor(v, off);
-      if ((threadIdx.x & 63) < G) sums[wave][side][l.e0 + e] = v;
+      for (int off = G; off < 64; off *= 2) {
+        va += __shfl_xor(va, off);
+        vb += __shfl_xor(vb, off);
+      }
+      if ((threadIdx.x & 63) < G) {
+        sums[wave][side][first_at<INTER>(l, i)] = va;
+        sums[wave][side][second_at<INTER>(l, i)] = vb;
+      }
     }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) {

@@ -249,6 +249,36 @@ def test_matches_the_norm_and_rope_it_replaces(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("inter", [True, False])
+@pytest.mark.parametrize("d", [64, 50])
+@pytest.mark.parametrize("sections", [
+    [1, 1, -2], [0, 3, -3], [-2, 1, 1], [2, 0, 0, -2], [-0, 0], [5, 9, 1, -15]])
+def test_short_and_empty_sections(sections, d, inter, device):
+    _skip(device)
+    half = d // 2
+    # the negative entry takes the rest of the pairs
+    rest = half - sum(n for n in sections if n > 0)
+    sec = [n if n > 0 else 0 for n in sections]
+    sec[min(range(len(sections)), key=lambda i: sections[i])] = rest
+    (q, k, qw, kw, cos, sin, _, dq, dk), _ = _case(
+        2, 5, 3, 1, d, d // 2 * 2, torch.bfloat16, torch.float32,
+        device=device)
+    g = torch.Generator().manual_seed(8)
+    pos = torch.randint(0, 300, (len(sec), 2, 5), generator=g).to(device)
+    pos[-1] = pos[0]  # first and last axis at the same position
+    for v in (q, k, qw, kw):
+        v.requires_grad_(True)
+    y = qk_norm_rope(q, k, qw, kw, cos, sin, positions=pos, sections=sec,
+                     interleaved=inter)
+    grads = torch.autograd.grad(y, (q, k), (dq, dk))
+    for out, x, w, dy, dx in ((y[0], q, qw, dq, grads[0]),
+                              (y[1], k, kw, dk, grads[1])):
+        oy, odx, _ = _oracle(x, w, dy, cos, sin, pos, sec, 1e-6, inter)
+        _close(out, oy, torch.bfloat16, "y")
+        _close(dx, odx, torch.bfloat16, "dx")
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("d", [64, 100])
 def test_edges(d, device):
     _skip(device)
