@@ -215,12 +215,13 @@ __global__ __launch_bounds__(kThreads) void bwd_any_kernel(
 // queries, then keys.  The angles and positions of a token are read once.
 // Needs D in eights and pairs in fours (see fits()), but no alignment.
 //
-// Bound by memory.  Heads of more than elem::kCached are written past the
-// caches (NT): 16384 tokens of 32 + 8 heads of 128 in bf16 take 58 us forward
-// (336 MB, 5.7 TB/s; 66 us through the caches) and 90 + 4 us backward
-// (503 MB, 5.6 TB/s; 110 us).  The backward keeps dw in registers over all
-// rows of a wave; 1024 blocks hide its latency (512: 126 us) and more of them
-// only lengthen the sum over blocks (4096: 10 us).
+// Bound by memory: 16384 tokens of 32 + 8 heads of 128 in bf16 take 58 us
+// forward (336 MB, 5.8 TB/s) and 86 + 4 us backward (503 MB, 5.8 TB/s).
+// Heads of more than elem::kCached are written past the caches (NT): through
+// them 66 against 58 us and 110 against 90 us.  The backward keeps dw in
+// registers over all rows of a wave; 1024 blocks hide its latency (512: 126
+// against 90 us), more of them only lengthen the sum over blocks (4096: 10
+// us), and reading a head ahead gained nothing.
 constexpr int kRun = 8;
 
 template <int CTRL>
