@@ -1,19 +1,20 @@
 // Log-probabilities of given tokens, and the losses built on them (MI355X).
 //
-// For a row of logits x and a token t, with M = max x:
-//   lp = x_t - M - log sum_j exp(x_j - M)
-//   d lp / d x_j = [j = t] - exp(x_j - M) / sum
+// For a row of logits x and a token t:
+//   lp = x_t - lse,  lse = log sum_j exp(x_j)
+//   d lp / d x_j = [j = t] - exp(x_j - lse)
 // Every loss here is a function of the lp alone, so a step is three passes
-// over memory: the forward reads the logits once (running maximum and sum),
+// over memory: the forward reads the logits once (running reference and sum),
 // a finishing kernel turns the row statistics into lp, the loss and each
 // row's d loss / d lp, and the backward reads the logits once more and
 // writes the gradient.  Rows whose target is ignored are not read, nor, in
 // the backward, rows whose coefficient is zero (clipped tokens): their
 // gradient is written as zeros.
 //
-// The sum of exponentials is kept in fp32; what follows it (log, differences
-// to other log-probabilities, sums over tokens) is done in fp64, because the
-// losses take small differences of large sums.
+// Exponentials are fp32; their long sums and what follows them (log,
+// differences to other log-probabilities, sums over tokens) are fp64, because
+// the losses take small differences of large sums.  For the same reason the
+// sums must not be off the same way in every row: see Part.
 
 #include <hip/hip_runtime.h>
 
@@ -24,7 +25,6 @@ namespace {
 using elem::kVec;
 
 constexpr int kThreads = 256;
-constexpr float kLowest = -3.402823466e38f;  // finite
 
 struct Shape {
   long rows, vocab;        // rows = outer * inner
@@ -43,19 +43,90 @@ __device__ __forceinline__ bool is_live(long t, long vocab, long ignore) {
   return t != ignore && t >= 0 && t < vocab;
 }
 
-// exp(d), d <= 0.  log2 e comes in two parts: with the rounded constant alone
-// every term would be off the same way (1.3e-8 |d|), and that does not
-// average out over the tokens of a sequence.
-__device__ __forceinline__ float exp_neg(float d) {
-  const float t = d * 1.925963033500011e-08f;
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.4426950216293335f, t));
+// log2 e: rounded, what that leaves, and with 16 bits, so that its product
+// with a bf16 number is exact.
+constexpr float kLog2e = 1.4426950216293335f;
+constexpr float kLog2eLow = 1.925963033500011e-08f;
+constexpr float kLog2e16 = 47274.f / 32768.f;
+constexpr double kLn2 = 0.6931471805599453;
+// v_exp_f32 comes out 3.2e-9 low on the average of its arguments.
+constexpr double kExpBias = 3.2e-9;
+
+// exp(d)
+__device__ __forceinline__ float exp_of(float d) {
+  return __builtin_amdgcn_exp2f(
+      __builtin_fmaf(d, kLog2e, d * kLog2eLow));
 }
 
-// (M, sum) of two pieces of a row.
-__device__ __forceinline__ void join(float& m, float& s, float mo, float so) {
-  const float top = fmaxf(m, mo);
-  s = s * exp_neg(m - top) + so * exp_neg(mo - top);
-  m = top;
+// A part of a row: its maximum, and  sum = sum_j 2^(x_j B - k).  Sequences add
+// the lp of many tokens up, so what matters is that the sums are not off the
+// same way in every row:
+// * k is a whole number near max B, so parts join by exact powers of two; with
+//   the maximum as the reference each joining multiplies a rounded
+//   exponential in;
+// * B is log2 e a share kCut short, 1.3e-8 by its rounding to fp32.  A bf16 row
+//   is a few hundred values whose products with that round alike in every
+//   row (1e-8 of lp): there B has 16 bits, the products are exact and kCut is
+//   4.9e-6.  Both are given back by
+//     log sum exp(x) = log sum exp((1 - kCut) x) + kCut E[x] + O(kCut^2 Var),
+//   E[x] = moment / sum;
+// * a few values are added in fp32, in pairs, and these sums in fp64: a long
+//   fp32 sum loses many small terms.
+// Over 20000 rows of 32000 values the mean of lp is off by less than 3e-9.
+struct Part {
+  double sum;
+  float max, k, moment, unused;
+};
+
+template <bool BF16>
+constexpr float kBase = BF16 ? kLog2e16 : kLog2e;
+template <bool BF16>
+constexpr double kCut = 1. - (double)kBase<BF16> * kLn2;
+
+// From these maxima on the next smaller value of the type lies 32 or more
+// below: only the values equal to the maximum count, and sum is their number.
+// It keeps x B within what fp32 resolves, and kCut E[x] small.
+template <bool BF16>
+constexpr float kHuge = BF16 ? 8192.f : 536870912.f;
+constexpr float kLeast = -1e9f;  // first k
+
+__device__ __forceinline__ Part nothing() {
+  return Part{0., -__builtin_huge_valf(), kLeast, 0.f, 0.f};
+}
+
+template <bool BF16>
+__device__ __forceinline__ bool is_huge(float m) {
+  return fabsf(m) >= kHuge<BF16> && fabsf(m) <= 3.402823466e38f;
+}
+
+__device__ __forceinline__ float shifted(float v, float by) {
+  return __builtin_ldexpf(v, (int)fmaxf(by, -2000.f));
+}
+__device__ __forceinline__ double shifted(double v, float by) {
+  return __builtin_ldexp(v, (int)fmaxf(by, -2000.f));
+}
+
+template <bool BF16>
+__device__ __forceinline__ void join(Part& p, const Part& q) {
+  if (is_huge<BF16>(p.max) || is_huge<BF16>(q.max)) {
+    // the larger maximum takes all; NaN stays
+    const double seen = p.sum + q.sum;
+    if (seen != seen) p.sum = seen;
+    else if (p.max == q.max) p.sum = seen;
+    else if (q.max > p.max) p = q;
+    p.max = fmaxf(p.max, q.max);
+    return;
+  }
+  const float k = fmaxf(p.k, q.k);
+  p.sum = shifted(p.sum, p.k - k) + shifted(q.sum, q.k - k);
+  p.moment = shifted(p.moment, p.k - k) + shifted(q.moment, q.k - k);
+  p.k = k;
+  p.max = fmaxf(p.max, q.max);
+}
+
+__device__ __forceinline__ Part from_lane(const Part& p, int off) {
+  return Part{__shfl_xor(p.sum, off), __shfl_xor(p.max, off),
+              __shfl_xor(p.k, off), __shfl_xor(p.moment, off), 0.f};
 }
 
 // Elements of `row` up to the first 16-byte boundary.
@@ -65,23 +136,70 @@ __device__ __forceinline__ int head_of(const T* p) {
          (int)sizeof(T);
 }
 
-// One value, or a few at once, into a thread's (M, sum).  M starts at the
-// lowest finite value, so -inf adds exp(-inf) = 0 and never meets -inf - -inf;
-// +inf and NaN make the sum NaN.
-template <int N>
-__device__ __forceinline__ void take(const float (&v)[N], float& m,
-                                     float& sum) {
+// 2^(x B - k)
+template <bool BF16>
+__device__ __forceinline__ float term(float x, float k) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kBase<BF16>, -k));
+}
+
+// One value, or a few at once, into a thread's part.  -inf adds 0; +inf and
+// NaN make the sum NaN.
+template <bool BF16, int N>
+__device__ __forceinline__ void take(const float (&v)[N], Part& p) {
   float top = v[0];
   #pragma unroll
   for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
-  if (top > m) {
-    sum *= exp_neg(m - top);
-    m = top;
+  p.max = fmaxf(p.max, top);
+  const float k = ceilf(top * kLog2e);
+  if (k > p.k) {
+    p.sum = shifted(p.sum, p.k - k);
+    p.moment = shifted(p.moment, p.k - k);
+    p.k = k;
   }
-  float add = 0.f;
+  float sum[N], moment = 0.f;
   #pragma unroll
-  for (int e = 0; e < N; ++e) add += exp_neg(v[e] - m);
-  sum += add;
+  for (int e = 0; e < N; ++e) {
+    const float x = sum[e] = term<BF16>(v[e], p.k);
+    // a masked value must not meet 0 * inf
+    moment = __builtin_fmaf(x, fmaxf(v[e], -1e30f), moment);
+  }
+  #pragma unroll
+  for (int half = N / 2; half > 0; half /= 2)
+    #pragma unroll
+    for (int e = 0; e < half; ++e) sum[e] += sum[e + half];
+  p.sum += (double)sum[0];
+  p.moment += moment;
+}
+
+// What the backward needs of a row is saved as four floats: its maximum R,
+// exp(R - lse), lp and the row's coefficient.
+struct RowLp {
+  float ref, inv;
+  double lp;
+};
+
+template <bool BF16>
+__device__ __forceinline__ RowLp finish(const Part& p, float xt) {
+  RowLp r;
+  if (is_huge<BF16>(p.max)) {
+    // the difference first: a sum would lose the logarithm
+    r.ref = p.max;
+    r.inv = (float)(1. / p.sum);
+    r.lp = ((double)xt - (double)p.max) - log(p.sum);
+    return r;
+  }
+  // lse - max, from the largest term in fp64 and what the others add to it: a
+  // token that is almost certain keeps its lp, and the bias is the others'
+  const double top =
+      exp2((double)p.max * (double)kBase<BF16> - (double)p.k);
+  const double rest = p.sum - (double)term<BF16>(p.max, p.k);
+  double over = log1p(rest * (1. + kExpBias) / top);
+  if (rest > 0.)
+    over += kCut<BF16> * ((double)p.moment / p.sum - (double)p.max);
+  r.ref = p.max;
+  r.inv = (float)exp(-over);
+  r.lp = ((double)xt - (double)p.max) - over;
+  return r;
 }
 
 // One block for each (row, piece of the vocabulary): stats[row, piece].
@@ -97,10 +215,11 @@ __device__ __forceinline__ void take(const float (&v)[N], float& m,
 template <typename T, int THREADS, bool FINISH>
 __global__ __launch_bounds__(THREADS) void row_stats_kernel(
     const T* __restrict__ logits, const long* __restrict__ target,
-    float2* __restrict__ stats, float* __restrict__ picked,
+    Part* __restrict__ stats, float* __restrict__ picked,
     unsigned* __restrict__ ticket, Shape s, long ignore, int pieces,
     long piece, float4* __restrict__ saved, float* __restrict__ lp) {
   constexpr int V = kVec<T>;
+  constexpr bool kBf16 = std::is_same_v<T, __bf16>;
   using Vec = elem::vec<T, V>;
   const long row = blockIdx.x;
   const int part = blockIdx.y;
@@ -120,7 +239,7 @@ __global__ __launch_bounds__(THREADS) void row_stats_kernel(
   const int body = (n - head) / V;
   const bool mine = threadIdx.x == 0 && t >= begin && t < begin + n;
   const float xt = mine ? (float)x[t - begin] : 0.f;
-  float m = kLowest, sum = 0.f;
+  Part p = nothing();
   const T* xv = x + head;
   int i = threadIdx.x;
   for (; i + 3 * THREADS < body; i += 4 * THREADS) {
@@ -131,72 +250,88 @@ __global__ __launch_bounds__(THREADS) void row_stats_kernel(
     float v[4 * V];
     #pragma unroll
     for (int e = 0; e < 4 * V; ++e) v[e] = (float)w[e / V][e % V];
-    take(v, m, sum);
+    take<kBf16>(v, p);
   }
   for (; i < body; i += THREADS) {
     const Vec w = elem::load<false, V>(xv + i * V);
     float v[V];
     #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = (float)w[e];
-    take(v, m, sum);
+    take<kBf16>(v, p);
   }
   const int rest = n - body * V;  // head and tail
   if ((int)threadIdx.x < rest) {
     const int at = (int)threadIdx.x < head ? (int)threadIdx.x
                                            : (int)threadIdx.x + body * V;
     const float v[1] = {(float)x[at]};
-    take(v, m, sum);
+    take<kBf16>(v, p);
   }
+  // one reference for the block, then plain sums
+  __shared__ float tops[THREADS / 64], moments[THREADS / 64];
+  __shared__ double sums[THREADS / 64];
+  float top = p.max;
   #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
-    join(m, sum, __shfl_xor(m, off), __shfl_xor(sum, off));
-  __shared__ float2 part_stats[THREADS / 64];
-  if ((threadIdx.x & 63) == 0)
-    part_stats[threadIdx.x >> 6] = make_float2(m, sum);
+    top = fmaxf(top, __shfl_xor(top, off));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  #pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) top = fmaxf(top, tops[w]);
+  const float k = fmaxf(ceilf(top * kLog2e), kLeast);
+  if (is_huge<kBf16>(top)) {
+    p = nothing();
+    for (int at = threadIdx.x; at < n; at += THREADS) {
+      const float v = (float)x[at];
+      p.sum += v != v ? v : v == top ? 1.f : 0.f;
+    }
+  } else {
+    p.sum = shifted(p.sum, p.k - k);
+    p.moment = shifted(p.moment, p.k - k);
+  }
+  #pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    p.sum += __shfl_xor(p.sum, off);
+    p.moment += __shfl_xor(p.moment, off);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sums[threadIdx.x >> 6] = p.sum;
+    moments[threadIdx.x >> 6] = p.moment;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     #pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w)
-      join(m, sum, part_stats[w].x, part_stats[w].y);
+    for (int w = 1; w < THREADS / 64; ++w) {
+      p.sum += sums[w];
+      p.moment += moments[w];
+    }
+    p.max = top;
+    p.k = k;
     if (!FINISH) {
-      stats[row * pieces + part] = make_float2(m, sum);
+      stats[row * pieces + part] = p;
       if (mine) picked[row] = xt;
       return;
     }
-    const double l = (double)xt - (double)m - log((double)sum);
-    lp[row] = (float)l;
-    if (saved) saved[row] = make_float4(m, 1.f / sum, (float)l, 1.f);
+    const RowLp r = finish<kBf16>(p, xt);
+    lp[row] = (float)r.lp;
+    if (saved) saved[row] = make_float4(r.ref, r.inv, (float)r.lp, 1.f);
   }
 }
-
-struct RowLp {
-  float m, inv;  // maximum, 1 / sum
-  double lp;
-};
 
 // Joins the pieces of a row in their order.
-__device__ __forceinline__ RowLp row_lp(const float2* __restrict__ stats,
+template <bool BF16>
+__device__ __forceinline__ RowLp row_lp(const Part* __restrict__ stats,
                                         const float* __restrict__ picked,
                                         long row, int pieces) {
-  float2 a = stats[row * pieces];
-  #pragma unroll 8
-  for (int p = 1; p < pieces; ++p) {
-    const float2 b = stats[row * pieces + p];
-    join(a.x, a.y, b.x, b.y);
-  }
-  RowLp r;
-  r.m = a.x;
-  r.inv = 1.f / a.y;
-  r.lp = (double)picked[row] - (double)a.x - log((double)a.y);
-  return r;
+  Part a = stats[row * pieces];
+  #pragma unroll 4
+  for (int p = 1; p < pieces; ++p) join<BF16>(a, stats[row * pieces + p]);
+  return finish<BF16>(a, picked[row]);
 }
 
-// What the backward needs of a row is saved as four floats: M, 1 / sum, lp
-// and the row's coefficient.
-
 // A wave for each row, of which there are few and the pieces many.
+template <bool BF16>
 __global__ __launch_bounds__(64) void lp_finish_kernel(
-    const long* __restrict__ target, const float2* __restrict__ stats,
+    const long* __restrict__ target, const Part* __restrict__ stats,
     const float* __restrict__ picked, float4* __restrict__ saved,
     float* __restrict__ lp, Shape s, long ignore, int pieces) {
   const long row = blockIdx.x;
@@ -208,18 +343,15 @@ __global__ __launch_bounds__(64) void lp_finish_kernel(
     }
     return;
   }
-  float m = kLowest, sum = 0.f;
-  for (int p = lane; p < pieces; p += 64) {
-    const float2 b = stats[row * pieces + p];
-    join(m, sum, b.x, b.y);
-  }
+  Part p = nothing();
+  for (int i = lane; i < pieces; i += 64)
+    join<BF16>(p, stats[row * pieces + i]);
   #pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    join(m, sum, __shfl_xor(m, off), __shfl_xor(sum, off));
+  for (int off = 32; off > 0; off >>= 1) join<BF16>(p, from_lane(p, off));
   if (lane == 0) {
-    const double l = (double)picked[row] - (double)m - log((double)sum);
-    lp[row] = (float)l;
-    if (saved) saved[row] = make_float4(m, 1.f / sum, (float)l, 1.f);
+    const RowLp r = finish<BF16>(p, picked[row]);
+    lp[row] = (float)r.lp;
+    if (saved) saved[row] = make_float4(r.ref, r.inv, (float)r.lp, 1.f);
   }
 }
 
@@ -262,8 +394,9 @@ struct PolicyArgs {
 // rho = exp(lp - old);  token loss = -min(rho A, clip(rho) A)
 //                                    + kl (e^d - d - 1),  d = ref - lp
 // The partial sums of the blocks are added in their order by the last one.
+template <bool BF16>
 __global__ __launch_bounds__(kThreads) void policy_finish_kernel(
-    const long* __restrict__ target, const float2* __restrict__ stats,
+    const long* __restrict__ target, const Part* __restrict__ stats,
     const float* __restrict__ picked, const float* __restrict__ old_lp,
     const float* __restrict__ adv, const float* __restrict__ ref_lp,
     float4* __restrict__ saved, double* __restrict__ partial,
@@ -276,7 +409,7 @@ __global__ __launch_bounds__(kThreads) void policy_finish_kernel(
     const long t = target[row];
     float4 keep = make_float4(0.f, 0.f, 0.f, 0.f);
     if (is_live(t, s.vocab, ignore)) {
-      const RowLp r = row_lp(stats, picked, row, pieces);
+      const RowLp r = row_lp<BF16>(stats, picked, row, pieces);
       const double rho = exp(r.lp - (double)old_lp[row]);
       const double A = (double)adv[row];
       const double free = rho * A;
@@ -292,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void policy_finish_kernel(
         coef += a.kl * (1. - exp(d));
       }
       count = 1.;
-      keep = make_float4(r.m, r.inv, (float)r.lp, (float)coef);
+      keep = make_float4(r.ref, r.inv, (float)r.lp, (float)coef);
     }
     saved[row] = keep;
   }
@@ -324,8 +457,9 @@ constexpr int kPairThreads = 512;
 //   loss = (1 - eps) softplus(-h) + eps softplus(h).
 // Rows of the chosen sequence get d loss / d lp = slope[pair], of the rejected
 // one its negative; the mean over the pairs is in it.
+template <bool BF16>
 __global__ __launch_bounds__(kPairThreads) void prefer_finish_kernel(
-    const long* __restrict__ target, const float2* __restrict__ stats,
+    const long* __restrict__ target, const Part* __restrict__ stats,
     const float* __restrict__ picked, const float* __restrict__ ref_lp,
     float4* __restrict__ saved, double* __restrict__ partial,
     unsigned* __restrict__ ticket, float* __restrict__ loss,
@@ -339,11 +473,11 @@ __global__ __launch_bounds__(kPairThreads) void prefer_finish_kernel(
     const long row = side ? (pair + pairs - 1) * seq + i : pair * seq + i;
     float4 keep = make_float4(0.f, 0.f, 0.f, 0.f);
     if (is_live(target[row], s.vocab, ignore)) {
-      const RowLp r = row_lp(stats, picked, row, pieces);
+      const RowLp r = row_lp<BF16>(stats, picked, row, pieces);
       const double d = r.lp - (double)ref_lp[row];
       sums[0] += side ? 0. : d;
       sums[1] += side ? d : 0.;
-      keep = make_float4(r.m, r.inv, (float)r.lp, side ? -1.f : 1.f);
+      keep = make_float4(r.ref, r.inv, (float)r.lp, side ? -1.f : 1.f);
     }
     saved[row] = keep;
   }
@@ -376,7 +510,7 @@ struct Scale {
   long rows, groups;
 };
 
-// dx_j = c ([j = t] - exp(x_j - M) / sum),  c = coef * up * scale.
+// dx_j = c ([j = t] - exp(x_j - R) exp(R - lse)),  c = coef * up * scale.
 //
 // Bound by memory: 8192 rows of 128256 bf16, 60 % of them read, take 575 us
 // (3.4 GB, 5.8 TB/s).  Blocks of 1024 threads with four accesses each beat
@@ -422,7 +556,7 @@ __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
   const auto slope = [&](const Vec& w) {
     Vec o;
     #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = (T)(k * exp_neg((float)w[e] - r.x));
+    for (int e = 0; e < V; ++e) o[e] = (T)(k * exp_of((float)w[e] - r.x));
     return o;
   };
   int i = threadIdx.x;
@@ -438,7 +572,7 @@ __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
   for (; i < body; i += THREADS)
     elem::store<NT, V>(dv + i * V, slope(elem::load<NT, V>(xv + i * V)));
   if ((int)threadIdx.x < rest)
-    dx[lone] = (T)(k * exp_neg((float)x[lone] - r.x));
+    dx[lone] = (T)(k * exp_of((float)x[lone] - r.x));
   __syncthreads();  // the target's own value last
   if (threadIdx.x == 0 && at >= 0 && at < n) dx[at] = at_target;
 }
@@ -538,16 +672,16 @@ struct Scratch {
   at::Tensor store;
   double* partial;
   unsigned* ticket;
-  float2* stats;
+  Part* stats;
   float* picked;
   Scratch(const at::Tensor& like, long partials, const Call& c) {
-    const long n = partials + 1 + c.s.rows * c.pieces;
-    store = at::empty({n * 8 + c.s.rows * 4},
+    const long n = partials + 1;
+    store = at::empty({n * 8 + c.s.rows * (c.pieces * (long)sizeof(Part) + 4)},
                       like.options().dtype(at::kByte));
     partial = (double*)store.data_ptr();
     ticket = (unsigned*)(partial + partials);
-    stats = (float2*)(partial + partials + 1);
-    picked = (float*)(partial + n);
+    stats = (Part*)(partial + n);
+    picked = (float*)(stats + c.s.rows * c.pieces);
   }
 };
 
@@ -644,7 +778,8 @@ at::Tensor logprobs_forward(const at::Tensor& logits,
       const Scratch tmp(logits, 0, c);
       launch_stats<T>(logits, target, c, tmp);
       hipLaunchKernelGGL(
-          lp_finish_kernel, dim3((unsigned)c.s.rows), dim3(64), 0,
+          (lp_finish_kernel<std::is_same_v<T, __bf16>>),
+          dim3((unsigned)c.s.rows), dim3(64), 0,
           elem::stream(), target.data_ptr<long>(), tmp.stats, tmp.picked,
           keep, lp.data_ptr<float>(), c.s, ignore, c.pieces);
     }
@@ -686,7 +821,8 @@ at::Tensor policy_forward(const at::Tensor& logits, const at::Tensor& target,
   STOKE_ELEM_SWITCH(logits.scalar_type(), "policy_loss", {
     launch_stats<T>(logits, target, c, tmp);
     hipLaunchKernelGGL(
-        policy_finish_kernel, dim3((unsigned)blocks), dim3(kThreads), 0,
+        (policy_finish_kernel<std::is_same_v<T, __bf16>>),
+        dim3((unsigned)blocks), dim3(kThreads), 0,
         elem::stream(), target.data_ptr<long>(), tmp.stats, tmp.picked,
         old_lp.data_ptr<float>(),
         adv.data_ptr<float>(),
@@ -746,7 +882,8 @@ variable_list preference_forward(const at::Tensor& logits,
   STOKE_ELEM_SWITCH(logits.scalar_type(), "preference_loss", {
     launch_stats<T>(logits, target, c, tmp);
     hipLaunchKernelGGL(
-        prefer_finish_kernel, dim3((unsigned)pairs), dim3(kPairThreads), 0,
+        (prefer_finish_kernel<std::is_same_v<T, __bf16>>),
+        dim3((unsigned)pairs), dim3(kPairThreads), 0,
         elem::stream(), target.data_ptr<long>(), tmp.stats, tmp.picked,
         ref_lp.data_ptr<float>(),
         (float4*)saved.data_ptr(), tmp.partial, tmp.ticket,
