@@ -243,8 +243,8 @@ __device__ __forceinline__ RowLp finish(const Part& p, float xt) {
 // finishing kernels would meet another one for each row.  With FINISH (one
 // piece a row) a row's lp is written here.
 //
-// Bound by memory: 8192 rows of 128256 bf16, 60 % of them read, take 215 us
-// (1.26 GB, 5.9 TB/s).  A thread takes 32 values between two looks at its
+// Bound by memory: 8192 rows of 128256 bf16, 60 % of them read, take 224 us
+// (1.26 GB, 5.6 TB/s).  A thread takes 32 values between two looks at its
 // maximum; the loads stay in the caches for the backward.
 template <typename T, int THREADS, bool FINISH>
 __global__ __launch_bounds__(THREADS) void row_stats_kernel(
@@ -552,8 +552,8 @@ struct Scale {
 
 // dx_j = c ([j = t] - exp(x_j - R) exp(R - lse)),  c = coef * up * scale.
 //
-// Bound by memory: 8192 rows of 128256 bf16, 60 % of them read, take 575 us
-// (3.4 GB, 5.8 TB/s).  Blocks of 1024 threads with four accesses each beat
+// Bound by memory: 8192 rows of 128256 bf16, 60 % of them read, take 567 us
+// (3.4 GB, 5.9 TB/s).  Blocks of 1024 threads with four accesses each beat
 // 256 threads (616 against 670 us for the same rows).
 template <typename T, int THREADS, bool NT>
 __global__ __launch_bounds__(THREADS) void lp_bwd_kernel(
