@@ -700,9 +700,10 @@ at::Tensor per_token(const at::Tensor& v, const at::Tensor& target,
   return x.contiguous();
 }
 
-bool wants_grad(const at::Tensor& x) {
-  if (!at::GradMode::is_enabled() || !x.requires_grad()) return false;
-  elem::check_capture({x});
+// Of the logits as they were given: a copy of a leaf is not a leaf.
+bool wants_grad(const at::Tensor& logits) {
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) return false;
+  elem::check_capture({logits});
   return true;
 }
 
@@ -969,7 +970,7 @@ at::Tensor token_logprobs(at::Tensor logits, at::Tensor target,
                           int64_t ignore) {
   check(logits, target, "token_logprobs");
   const auto x = rows_of(logits), t = target.contiguous();
-  if (!wants_grad(x)) return logprobs_forward(x, t, ignore, at::Tensor());
+  if (!wants_grad(logits)) return logprobs_forward(x, t, ignore, at::Tensor());
   return TokenLogprobs::apply(x, t, ignore);
 }
 
@@ -988,7 +989,7 @@ at::Tensor policy_loss(at::Tensor logits, at::Tensor target,
   const auto adv_rows = per_token(adv, target, "advantages");
   std::optional<at::Tensor> ref;
   if (kl != 0) ref = per_token(*ref_lp, target, "ref_logprobs");
-  if (wants_grad(x))
+  if (wants_grad(logits))
     return PolicyLoss::apply(x, t, old_rows, adv_rows, ref, 1. - clip_low,
                              1. + clip_high, kl, ignore);
   at::Tensor saved;
@@ -1011,7 +1012,7 @@ std::vector<at::Tensor> preference_loss(at::Tensor logits, at::Tensor target,
                     "0 <= label_smoothing <= 0.5, got ", beta, ", ", eps);
   const auto x = rows_of(logits), t = target.contiguous();
   const auto ref = per_token(ref_lp, target, "ref_logprobs");
-  if (wants_grad(x))
+  if (wants_grad(logits))
     return PreferenceLoss::apply(x, t, ref, beta, eps, ignore);
   at::Tensor saved;
   return preference_forward(x, t, ref, beta, eps, ignore, saved);

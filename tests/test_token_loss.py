@@ -560,6 +560,29 @@ def test_gpu_capture_over_a_live_graph_of_the_same_leaf_is_refused():
 
 
 @pytest.mark.gpu
+def test_gpu_capture_over_a_live_graph_of_a_transposed_leaf_is_refused():
+    """Logits that are copied first: the leaf is behind the copy."""
+    _skip("cuda")
+    x, t = _inputs((2, 3, 50), torch.float32, "cuda", keep=1.0)
+    x = x.transpose(1, 2).contiguous().transpose(1, 2).requires_grad_(True)
+    assert x.is_leaf and x.stride(-1) != 1
+    v = torch.zeros(2, 3, device="cuda")
+    alive = token_logprobs(x, t)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for call in (lambda: token_logprobs(x, t),
+                     lambda: fused_policy_loss(x, t, v, v),
+                     lambda: fused_preference_loss(x, t, v)):
+            with pytest.raises(RuntimeError, match="drop that graph"):
+                call()
+        with torch.no_grad():
+            out = token_logprobs(x, t)
+    graph.replay()
+    assert torch.equal(out, alive.detach())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("v", [50257, 131072])
 def test_gpu_logits_past_the_cached_size(v):
     """Large calls take other accesses and blocks: the same values."""
