@@ -4,7 +4,9 @@ here, HIP kernels in the gpu tier)."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
+from stoke import ops
 from stoke.nn import StokeQKNorm, StokeRMSNorm, qk_norm_rope
 from stoke.nn.rope import apply_rope
 
@@ -383,6 +385,34 @@ def test_refusals(device):
     for call in cases:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_is_refused_by_the_kernels(device):
+    """A tangent must not vanish; the extension sees it before the device."""
+    _skip(device)
+    if not ops.has_ext():
+        pytest.skip("extension not built")
+    (q, k, qw, kw, cos, sin, pos, _, _), _ = _case(
+        2, 6, 3, 1, 64, 64, torch.float32, torch.float32, device=device)
+    with fwd.dual_level():
+        for i in range(6):
+            args = [q, k, qw, kw, cos, sin]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            for grad in (False, True):
+                q.requires_grad_(grad)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    ops._require_ext().qk_norm_rope(*args, pos, None, 1e-6,
+                                                    True)
+                if device == "cuda":
+                    with pytest.raises(NotImplementedError):
+                        qk_norm_rope(*args, positions=pos)
+            q.requires_grad_(False)
+            if device == "cpu":
+                y, _ = qk_norm_rope(*args, positions=pos)
+                z = qk_norm_rope(*args, positions=pos)[1]
+                assert any(fwd.unpack_dual(o).tangent is not None
+                           for o in (y, z))
 
 
 @pytest.mark.gpu

@@ -4,7 +4,9 @@ formulas (torch path here, HIP kernels in the gpu tier)."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
+from stoke import ops
 from stoke.nn import fused_policy_loss, fused_preference_loss, token_logprobs
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -429,6 +431,65 @@ def test_refusals(device):
     for call in cases:
         with pytest.raises(ValueError):
             call()
+
+
+def _tangent_calls(x, t, v, dx):
+    """The losses with a forward-mode tangent in each of their inputs."""
+    return [
+        lambda: token_logprobs(dx(x), t),
+        lambda: fused_policy_loss(dx(x), t, v, v + 1),
+        lambda: fused_policy_loss(x, t, dx(v), v + 1),
+        lambda: fused_policy_loss(x, t, v, dx(v + 1)),
+        lambda: fused_policy_loss(x, t, v, v, dx(v), kl_coef=0.1),
+        lambda: fused_preference_loss(dx(x), t, v)[0],
+        lambda: fused_preference_loss(x, t, dx(v))[0],
+    ]
+
+
+def test_forward_mode_on_the_cpu():
+    x, t = _inputs((2, 3, 11), torch.float32, "cpu", keep=1.0)
+    x, v = x.double(), torch.zeros(2, 3).double()
+    with fwd.dual_level():
+        for call in _tangent_calls(
+                x, t, v, lambda y: fwd.make_dual(y, torch.ones_like(y))):
+            assert fwd.unpack_dual(call()).tangent is not None
+    for fn in (lambda y: token_logprobs(y, t),
+               lambda y: fused_policy_loss(y, t, v - 3, v + 1),
+               lambda y: fused_preference_loss(y, t, v)[0]):
+        assert torch.autograd.gradcheck(
+            fn, (x.clone().requires_grad_(True),), check_forward_ad=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_is_refused_by_the_kernels(device):
+    """A tangent must not vanish; the extension sees it before the device."""
+    _skip(device)
+    if not ops.has_ext():
+        pytest.skip("extension not built")
+    ext = ops._require_ext()
+    x = torch.zeros(2, 3, 5, device=device)
+    t = torch.zeros(2, 3, dtype=torch.int64, device=device)
+    v = torch.zeros(2, 3, device=device)
+    with fwd.dual_level():
+        def dx(y):
+            return fwd.make_dual(y, torch.ones_like(y))
+
+        calls = [
+            lambda: ext.token_logprobs(dx(x), t, IGN),
+            lambda: ext.policy_loss(dx(x), t, v, v, None, .2, .2, 0., IGN),
+            lambda: ext.policy_loss(x, t, dx(v), v, None, .2, .2, 0., IGN),
+            lambda: ext.policy_loss(x, t, v, dx(v), None, .2, .2, 0., IGN),
+            lambda: ext.policy_loss(x, t, v, v, dx(v), .2, .2, .1, IGN),
+            lambda: ext.preference_loss(dx(x), t, v, .1, 0., IGN),
+            lambda: ext.preference_loss(x, t, dx(v), .1, 0., IGN),
+        ]
+        if device == "cuda":
+            calls += _tangent_calls(x, t, v, dx)
+        for grad in (False, True):
+            x.requires_grad_(grad)
+            for call in calls:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
 
 
 @pytest.mark.gpu
