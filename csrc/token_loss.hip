@@ -532,8 +532,9 @@ __global__ __launch_bounds__(kPairThreads) void prefer_finish_kernel(
     slope[pair] = (float)(beta * dh / (double)pairs);
     rewards[pair] = (float)gain[0];
     rewards[pair + pairs] = (float)gain[1];
+    // without smoothing a margin of +inf costs nothing: not 0 * inf
     partial[pair] = (1. - eps) * (fmax(-h, 0.) + tail) +
-                    eps * (fmax(h, 0.) + tail);
+                    (eps > 0. ? eps * (fmax(h, 0.) + tail) : 0.);
   }
   if (!last_block(ticket)) return;
   double sum = 0.;

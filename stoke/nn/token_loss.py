@@ -181,6 +181,8 @@ def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
     good, bad = rewards.chunk(2)
     h = good - bad
     ls = torch.nn.functional.logsigmoid
-    loss = -((1 - label_smoothing) * ls(h) + label_smoothing * ls(-h))
+    loss = -(1 - label_smoothing) * ls(h)
+    if label_smoothing != 0:  # a margin of +inf: not 0 * inf
+        loss = loss - label_smoothing * ls(-h)
     dt = _result_dtype(logits)
     return loss.mean().to(dt), rewards.detach().to(dt)

@@ -325,6 +325,45 @@ def test_rows_without_a_distribution_are_nan(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_preference_at_an_infinite_margin(device):
+    _skip(device)
+    # one pair of two tokens, a constrained vocabulary: token 3 is at -inf
+    x = torch.randn(2, 2, 5, generator=_gen(8))
+    t = torch.full((2, 2), 2)
+    ref = torch.zeros(2, 2)
+
+    def call(side, smooth):
+        y, u = x.clone(), t.clone()
+        y[side, 0, 3] = -float("inf")
+        u[side, 0] = 3
+        y = y.to(device).requires_grad_(True)
+        loss, rewards = fused_preference_loss(
+            y, u.to(device), ref.to(device), beta=0.3, label_smoothing=smooth)
+        g, = torch.autograd.grad(loss, y)
+        assert float(rewards[side]) == -float("inf")
+        assert torch.isfinite(rewards[1 - side])
+        return float(loss.detach()), g.cpu().double(), y
+
+    # the rejected one is impossible: -log sigmoid(+inf) = 0, and flat
+    loss, g, _ = call(1, 0.0)
+    assert loss == 0.0
+    assert bool((g == 0).all())
+    # with smoothing the second term is infinite, its slope is not: d / dh of
+    # -eps log sigmoid(-h) is eps sigmoid(h) = eps
+    for side, smooth, slope in ((1, 0.1, 0.1), (0, 0.0, -1.0), (0, 0.1, -0.9)):
+        loss, g, y = call(side, smooth)
+        assert loss == float("inf")
+        p = torch.softmax(y.detach().cpu().double(), -1)
+        hot = torch.zeros_like(p)
+        hot[..., 2] = 1
+        hot[side, 0] = torch.tensor([0.0, 0, 0, 1, 0])
+        c = torch.tensor([1.0, -1.0]).double()[:, None, None]
+        want = 0.3 * slope * c * (hot - p)
+        # |d| < 6: terms are off by (1.25 * 6 + 3) U, twice, and 5 sums
+        assert bool(((g - want).abs() <= 40 * U * 0.3).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_ratio_on_the_clip_and_beyond(device):
     _skip(device)
     # uniform over 4 tokens: lp = -log 4; rho = 1/2, 1, 2 with clip [1/2, 2]
