@@ -461,8 +461,10 @@ __global__ __launch_bounds__(kThreads) void policy_finish_kernel(
       double coef = clipped ? 0. : -free;
       if (ref_lp) {
         const double d = (double)ref_lp[row] - r.lp;
-        tok += a.kl * (exp(d) - d - 1.);
-        coef += a.kl * (1. - exp(d));
+        const double e = exp(d);
+        // a token that the policy rules out: not inf - inf
+        tok += a.kl * (d == __builtin_huge_val() ? e : e - d - 1.);
+        coef += a.kl * (1. - e);
       }
       count = 1.;
       keep = make_float4(r.ref, r.inv, (float)r.lp, (float)coef);

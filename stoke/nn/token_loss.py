@@ -138,7 +138,9 @@ def fused_policy_loss(logits: torch.Tensor, actions: torch.Tensor,
     if kl_coef != 0:
         ref = _per_token(ref_logprobs, actions, "ref_logprobs")
         d = ref[live].double() - lp
-        tok = tok + kl_coef * (d.exp() - d - 1)
+        # a token that the policy rules out costs inf: not inf - inf
+        tok = tok + kl_coef * torch.where(
+            d == float("inf"), d, d.exp() - d - 1)
     return (tok.sum() / max(1, tok.numel())).to(_result_dtype(logits))
 
 

@@ -325,6 +325,32 @@ def test_rows_without_a_distribution_are_nan(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_policy_on_a_token_that_it_rules_out(device):
+    _skip(device)
+    x = torch.randn(1, 2, 5, generator=_gen(8))
+    x[0, 0, 3] = -float("inf")
+    t = torch.tensor([[3, 2]], device=device)
+    x = x.to(device).requires_grad_(True)
+    v = torch.full((1, 2), -1.0, device=device)
+    # rho is 0: without the KL term only the other token counts
+    a = fused_policy_loss(x, t, v, v + 2)
+    ga, = torch.autograd.grad(a, x)
+    b = fused_policy_loss(x[:, 1:], t[:, 1:], v[:, 1:], v[:, 1:] + 2)
+    gb, = torch.autograd.grad(b, x)
+    assert abs(float(a.detach()) - float(b.detach()) / 2) <= 4 * U * abs(
+        float(b.detach()))
+    assert bool((ga[0, 0] == 0).all())
+    assert torch.allclose(ga[0, 1], gb[0, 1] / 2, rtol=8 * U, atol=0)
+    # with it the loss is infinite, as e^d is
+    loss = fused_policy_loss(x, t, v, v + 2, v, kl_coef=0.1)
+    assert float(loss.detach()) == float("inf")
+    # where the reference rules it out too there is no value
+    ref = v.clone()
+    ref[0, 0] = -float("inf")
+    assert torch.isnan(fused_policy_loss(x, t, v, v + 2, ref, kl_coef=0.1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_preference_at_an_infinite_margin(device):
     _skip(device)
     # one pair of two tokens, a constrained vocabulary: token 3 is at -inf
