@@ -11,15 +11,20 @@ wrapped block for not storing its activations — on MI355X the recompute is
 usually HBM-resident and cheap relative to the 288 GB it frees for larger
 batches/models.
 
-``save_bits=8`` keeps the wrapped block's input activations in 8 bits
-(``stoke.nn.act8``): half the bytes of a 16-bit checkpoint.  The forward runs
-on the exact inputs; the recompute starts from the values held.
+``save_bits=8`` keeps the wrapped block's input in 8 bits (``stoke.nn.act8``):
+half the bytes of a 16-bit checkpoint.  The forward runs on the exact input;
+the recompute starts from the values held.  The input is the first argument
+of the block's ``forward``; the others (masks, biases, tables, expressions of
+parameters, an encoder's output) stay as they are: a mask's -inf or lowest
+value would take the other values of its 32 along, and what several blocks
+share would be held once for each.
 
 Composes with the FSDP engine: the recompute re-fires the unit's
 forward-pre hook, which re-gathers the flat-param shard it needs.
 """
 
 import functools
+import inspect
 from typing import Callable, Optional
 
 import torch
@@ -65,21 +70,32 @@ class _FillIn(torch.autograd.Function):
 
 
 def _holds(t) -> bool:
-    # computed activations only: parameters, caller-held leaves, masks and
-    # tables stay alive elsewhere, so compressing them would add memory
+    # computed activations only: parameters and caller-held leaves stay alive
+    # elsewhere, so compressing them would add memory
     return (isinstance(t, torch.Tensor) and t.grad_fn is not None
             and t.dtype in (torch.bfloat16, torch.float16, torch.float32))
 
 
-def _checkpoint8(fn, args, kwargs):
-    """``checkpoint(fn, *args, **kwargs)`` with the activations among the
-    arguments held in 8 bits until the backward pass."""
+def _first_parameter(forward) -> Optional[str]:
+    """Name of the argument that holds a block's input."""
+    for p in inspect.signature(forward).parameters.values():
+        return p.name if p.kind is p.POSITIONAL_OR_KEYWORD else None
+    return None
+
+
+def _checkpoint8(fn, first, args, kwargs):
+    """``checkpoint(fn, *args, **kwargs)`` with the activation in the first
+    argument (by name, ``first``) held in 8 bits until the backward pass."""
     flat = list(args) + list(kwargs.values())
-    held = {i: (compress_activation(t), [t]) for i, t in enumerate(flat)
-            if _holds(t)}
+    x = args[0] if args else kwargs.get(first)
+    held = {}
+    if _holds(x):
+        # also where it comes again: the exact one must not stay alive
+        packed = compress_activation(x)
+        held = {i: (packed, [t]) for i, t in enumerate(flat) if t is x}
     kept = [_StandIn.apply(t) if i in held else t for i, t in enumerate(flat)]
     n, names = len(args), list(kwargs)
-    del flat, args, kwargs
+    del x, flat, args, kwargs
 
     def run(*vals):
         vals = [_FillIn.apply(t, *held[i]) if i in held else t
@@ -94,13 +110,14 @@ def _wrap_module(m: nn.Module, save_bits: int = 16) -> None:
     if getattr(m, _MARK, False):
         return
     inner_forward = m.forward
+    first = _first_parameter(inner_forward)
 
     @functools.wraps(inner_forward)
     def ckpt_forward(*args, **kwargs):
         if not torch.is_grad_enabled() or not m.training:
             return inner_forward(*args, **kwargs)
         if getattr(m, _BITS) == 8:
-            return _checkpoint8(inner_forward, args, kwargs)
+            return _checkpoint8(inner_forward, first, args, kwargs)
         return checkpoint(
             inner_forward, *args, use_reentrant=False, **kwargs
         )
@@ -120,8 +137,9 @@ def apply_activation_checkpointing(
     Default eligibility: any non-container child subtree holding at least
     ``min_params`` parameters (the same granularity the FSDP engine uses for
     shard units).  A custom ``predicate(name, module)`` overrides it.
-    ``save_bits=8`` holds the blocks' input activations in 8 bits (see the
-    module docstring); 16 keeps them as they are.
+    ``save_bits=8`` holds the blocks' inputs, the first argument of their
+    ``forward``, in 8 bits (see the module docstring); 16 keeps them as they
+    are.
     Returns the number of modules wrapped.
     """
     check_save_bits(save_bits)

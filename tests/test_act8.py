@@ -2,7 +2,9 @@
 """Activations held in 8 bits: the format, SwiGLU and the checkpoints that
 use it (CPU steps here, HIP kernels in the gpu tier) against float64."""
 
+import gc
 import math
+import weakref
 
 import pytest
 import torch
@@ -20,6 +22,15 @@ DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 # around a block of 32, around 16-byte pieces, several blocks of threads
 SIZES = [(1,), (31,), (32,), (33,), (5, 7), (3, 64), (2, 3, 100), (4, 4096),
          (257, 1367)]
+
+
+@pytest.fixture(autouse=True)
+def _collected(request):
+    """A wrapped module refers to itself: what it holds on the GPU must not
+    be freed in the middle of a test that counts memory."""
+    yield
+    if "checkpoint8" in request.node.name:
+        gc.collect()
 
 
 def _skip(device):
@@ -424,6 +435,76 @@ def test_gpu_checkpoint8_saves_memory_under_autocast():
     per = 8192 * d
     assert held[16] >= (n + 1) * 2 * per
     assert held[8] <= n * per * 33 / 32 + 2 * per + (1 << 22)
+
+
+class _Scores(torch.nn.Module):
+    """Attention over rows of x with an additive bias."""
+
+    def __init__(self, d):
+        super().__init__()
+        self.w = torch.nn.Parameter(torch.eye(d))
+
+    def forward(self, x, bias, kv=None):
+        kv = x if kv is None else kv
+        return x + torch.softmax(x @ self.w @ kv.t() + bias, -1) @ kv
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("mask", ["-inf", "lowest", "-1e4"])
+@pytest.mark.parametrize("by_name", [False, True])
+def test_checkpoint8_leaves_biases_and_masks_exact(by_name, mask, device):
+    """A learned bias with a causal mask has a grad_fn as activations do."""
+    _skip(device)
+    low = {"-inf": -float("inf"), "lowest": torch.finfo(torch.float32).min,
+           "-1e4": -1e4}[mask]
+    # inputs that 8 bits hold exactly: the gradients are bit-equal
+    x = (torch.randint(-127, 128, (8, 32),
+                       generator=torch.Generator().manual_seed(1)) / 64)
+    x[:, 0] = 1.75
+    rel = torch.randn(8, 8, generator=torch.Generator().manual_seed(2))
+    far = torch.full((8, 8), low).triu(1)
+    grads = []
+    for bits in (16, 8):
+        net = torch.nn.Sequential(_Scores(32)).to(device)
+        apply_activation_checkpointing(net, predicate=lambda n, m: True,
+                                       save_bits=bits)
+        leaf = x.float().to(device).requires_grad_(True)
+        bias = rel.clone().to(device).requires_grad_(True)
+        seen = bias + far.to(device)
+        args = dict(bias=seen, x=leaf * 1.0)
+        y = net[0](**args) if by_name else net[0](args["x"], seen)
+        y.square().sum().backward()
+        grads.append((leaf.grad, bias.grad, net[0].w.grad))
+    for a, b in zip(*grads):
+        assert torch.isfinite(b).all() and bool((a != 0).any())
+        assert torch.equal(a, b)
+
+
+def test_checkpoint8_input_that_comes_twice():
+    x = (torch.randint(-127, 128, (8, 32),
+                       generator=torch.Generator().manual_seed(1)) / 64)
+    x[:, 0] = 1.75
+    bias = torch.zeros(8, 8)
+    leaves = [x.clone().requires_grad_(True) for _ in range(3)]
+    nets = [_Scores(32), torch.nn.Sequential(_Scores(32))]
+    apply_activation_checkpointing(nets[1], predicate=lambda n, m: True,
+                                   save_bits=8)
+    y = nets[0](leaves[0], bias, kv=leaves[1])
+    y.square().sum().backward()
+    t = leaves[2] * 1.0
+    alive = weakref.ref(t)
+    z = nets[1][0](t, bias, kv=t)
+    del t
+    gc.collect()
+    assert alive() is None
+    assert torch.equal(z, y)
+    z.square().sum().backward()
+    assert torch.equal(nets[0].w.grad, nets[1][0].w.grad)
+    # the same parts (of x: the residual's 2 y and the rest) in another order
+    a, b = (v.grad.double() for v in leaves[:2])
+    size = a.abs() + b.abs() + 4 * y.detach().double().abs()
+    assert bool(((leaves[2].grad.double() - a - b).abs()
+                 <= 4 * 2.0 ** -24 * size).all())
 
 
 @pytest.mark.gpu
