@@ -41,6 +41,30 @@ _MARK = "_stoke_act_ckpt"
 _BITS = "_stoke_act_ckpt_bits"
 
 
+class _Held:
+    """An activation in 8 bits that comes back with its strides.
+
+    The values are held in the order of memory, those of an expanded size
+    once: a block may view its input in ways that its strides allow and
+    others do not, and products pick their layout by them."""
+
+    def __init__(self, x):
+        strides = x.stride()
+        self.shape = x.shape
+        self.order = sorted(range(x.dim()), key=lambda d: -strides[d])
+        for d in range(x.dim()):
+            if strides[d] == 0 and x.shape[d] > 1:
+                x = x.narrow(d, 0, 1)
+        self.packed = compress_activation(x.permute(self.order))
+
+    def restore(self):
+        x = restore_activation(self.packed)
+        back = [0] * x.dim()
+        for i, d in enumerate(self.order):
+            back[d] = i
+        return x.permute(back).expand(self.shape)
+
+
 class _StandIn(torch.autograd.Function):
     """A tensor of x's shape without its memory, through which the gradient
     for x flows; the checkpoint keeps it in x's place."""
@@ -62,7 +86,7 @@ class _FillIn(torch.autograd.Function):
     def forward(ctx, stand_in, held, exact):
         if exact:
             return exact.pop().detach()
-        return restore_activation(held)
+        return held.restore()
 
     @staticmethod
     def backward(ctx, grad):
@@ -91,7 +115,7 @@ def _checkpoint8(fn, first, args, kwargs):
     held = {}
     if _holds(x):
         # also where it comes again: the exact one must not stay alive
-        packed = compress_activation(x)
+        packed = _Held(x)
         held = {i: (packed, [t]) for i, t in enumerate(flat) if t is x}
     kept = [_StandIn.apply(t) if i in held else t for i, t in enumerate(flat)]
     n, names = len(args), list(kwargs)

@@ -507,6 +507,68 @@ def test_checkpoint8_input_that_comes_twice():
                  <= 4 * 2.0 ** -24 * size).all())
 
 
+class _Strides(torch.nn.Module):
+    def __init__(self, view):
+        super().__init__()
+        self.view, self.seen = view, []
+
+    def forward(self, x):
+        self.seen.append((x.shape, x.stride(), x.detach().clone()))
+        return torch.tanh(self.view(x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", [
+    "contiguous", "channels_last", "channels_last_3d", "transposed", "slice",
+    "expanded", "one", "scalar", "empty"])
+def test_checkpoint8_recompute_sees_the_layout_of_the_forward(name, device):
+    _skip(device)
+    shape = {"channels_last_3d": (2, 8, 3, 4, 5), "scalar": (),
+             "one": (3, 1, 5, 1), "empty": (0, 4, 5, 6)}.get(
+                 name, (2, 8, 6, 5))
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randint(-127, 128, shape, generator=g) / 64).to(device)
+    n, c = shape[0] if shape else 1, shape[1] if shape else 1
+
+    # each made from the leaf, with the view that these strides allow
+    make, view = {
+        "contiguous": (lambda t: t * 1.0, lambda t: t.view(n, -1)),
+        "channels_last": (
+            lambda t: (t * 1.0).contiguous(memory_format=torch.channels_last),
+            lambda t: t.permute(0, 2, 3, 1).view(-1, c)),
+        "channels_last_3d": (
+            lambda t: (t * 1.0).contiguous(
+                memory_format=torch.channels_last_3d),
+            lambda t: t.permute(0, 2, 3, 4, 1).view(-1, c)),
+        "transposed": (lambda t: (t.transpose(0, 3) * 1.0).contiguous()
+                       .transpose(0, 3),
+                       lambda t: t.transpose(0, 3).view(-1)),
+        "slice": (lambda t: torch.cat((t, t), -1)[..., :shape[-1]],
+                  lambda t: t.flatten(1, 2).view(n, -1, shape[-1])),
+        "expanded": (lambda t: (t[:, :1, :, :1] * 1.0).expand(shape),
+                     lambda t: t[:, :, :, 0]),
+        "one": (lambda t: t * 1.0, lambda t: t.view(-1)),
+        "scalar": (lambda t: t * 1.0, lambda t: t.view(1)),
+        "empty": (lambda t: t * 1.0, lambda t: t.view(0, 5)),
+    }[name]
+    grads = []
+    for bits in (16, 8):
+        net = torch.nn.Sequential(_Strides(view))
+        apply_activation_checkpointing(net, predicate=lambda n, m: True,
+                                       save_bits=bits)
+        leaf = x.clone().requires_grad_(True)
+        inp = make(leaf)
+        net[0](inp).square().sum().backward()
+        (s0, t0, v0), (s1, t1, v1) = net[0].seen
+        assert s0 == s1 == x.shape
+        if name != "slice":  # gaps are not kept
+            assert all(a == b for a, b, k in zip(t0, t1, x.shape) if k > 1)
+        # 32 of these values share a step of at most 1/64
+        assert torch.equal(v0, v1)
+        grads.append(leaf.grad)
+    assert torch.equal(*grads)
+
+
 @pytest.mark.gpu
 def test_gpu_replays_in_a_graph():
     _skip("cuda")
