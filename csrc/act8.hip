@@ -199,8 +199,9 @@ struct Rows {
   long g, u;
 };
 
-// y = silu(g) * u from the values as they come; g and u stay in 8 bits.
-template <typename T, bool NT>
+// y = silu(g) * u from the values as they come; with KEEP g and u stay in 8
+// bits.  Without a backward to come nothing else is computed or written.
+template <typename T, bool NT, bool KEEP>
 __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     const T* __restrict__ g, const T* __restrict__ u, T* __restrict__ y,
     signed char* __restrict__ qg, signed char* __restrict__ qu,
@@ -222,11 +223,12 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     place(i, ig, iu);
     load_run<NT>(g, ig, a);
     load_run<NT>(u, iu, b);
-    Bytes qa, qb;
-    const unsigned ea = pack_run(a, qa), eb = pack_run(b, qb);
     #pragma unroll
     for (int e = 0; e < kRun; ++e) o[e] = swiglu(a[e], b[e]);
     store_run<false>(y, i, o);
+    if (!KEEP) continue;
+    Bytes qa, qb;
+    const unsigned ea = pack_run(a, qa), eb = pack_run(b, qb);
     *(Bytes*)(qg + i) = qa;
     *(Bytes*)(qu + i) = qb;
     if ((threadIdx.x & 3) == 0) {
@@ -240,12 +242,13 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(
     place(i, ig, iu);
     const float a = i < n ? (float)g[ig] : 0.f;
     const float b = i < n ? (float)u[iu] : 0.f;
+    if (i < n) y[i] = (T)swiglu(a, b);
+    if (!KEEP) continue;
     const unsigned eg =
         block_exponent(half_wave_max(__float_as_uint(a) & 0x7fffffff));
     const unsigned eu =
         block_exponent(half_wave_max(__float_as_uint(b) & 0x7fffffff));
     if (i < n) {
-      y[i] = (T)swiglu(a, b);
       qg[i] = (signed char)quantize(a, eg);
       qu[i] = (signed char)quantize(b, eu);
     }
@@ -336,8 +339,9 @@ long row_step(const at::Tensor& x) {
   return step;
 }
 
+// held: what the backward needs, null where there is none.
 at::Tensor swiglu8_forward(const at::Tensor& gate, const at::Tensor& up,
-                           at::Tensor& held) {
+                           at::Tensor* held) {
   const c10::DeviceGuard guard(gate.device());
   const long n = gate.numel();
   Rows rows{0, 0, 0};
@@ -349,17 +353,22 @@ at::Tensor swiglu8_forward(const at::Tensor& gate, const at::Tensor& up,
   const at::Tensor g = rows.cols ? gate : gate.contiguous();
   const at::Tensor u = rows.cols ? up : up.contiguous();
   auto y = at::empty(g.sizes(), g.options());
-  held = at::empty({Held(nullptr, n).bytes}, g.options().dtype(at::kByte));
+  if (held)
+    *held = at::empty({Held(nullptr, n).bytes}, g.options().dtype(at::kByte));
   if (n == 0) return y;
-  const Held h(held.data_ptr(), n);
+  const Held h(held ? held->data_ptr() : nullptr, n);
   STOKE_ELEM_SWITCH(g.scalar_type(), "swiglu8", {
     const long first = first_of(n);
     with_caching(n * (long)sizeof(T), [&](auto nt) {
-      hipLaunchKernelGGL((swiglu8_fwd_kernel<T, nt>), grid_for(n, first),
-                         dim3(kThreads), 0, elem::stream(),
-                         (const T*)g.data_ptr(), (const T*)u.data_ptr(),
-                         (T*)y.data_ptr(), h.qg, h.qu, h.sg, h.su, n, first,
-                         rows);
+      const auto launch = [&](auto keep) {
+        hipLaunchKernelGGL((swiglu8_fwd_kernel<T, nt, keep>),
+                           grid_for(n, first), dim3(kThreads), 0,
+                           elem::stream(), (const T*)g.data_ptr(),
+                           (const T*)u.data_ptr(), (T*)y.data_ptr(), h.qg,
+                           h.qu, h.sg, h.su, n, first, rows);
+      };
+      if (held) launch(std::true_type{});
+      else launch(std::false_type{});
     });
   });
   return y;
@@ -388,7 +397,7 @@ struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& g,
                             const at::Tensor& u) {
     at::Tensor held;
-    auto y = swiglu8_forward(g, u, held);
+    auto y = swiglu8_forward(g, u, &held);
     ctx->save_for_backward({held});
     return y;
   }
@@ -460,6 +469,7 @@ at::Tensor act8_unpack(at::Tensor values, at::Tensor scales,
 
 // The entry point: checks its arguments, and has gradients for both.
 at::Tensor swiglu8(at::Tensor g, at::Tensor u) {
+  elem::refuse_tangents("swiglu(save_bits=8)", {g, u});
   TORCH_CHECK_VALUE(
       g.is_cuda() && g.sizes() == u.sizes() && g.device() == u.device() &&
           g.scalar_type() == u.scalar_type() &&
@@ -468,6 +478,8 @@ at::Tensor swiglu8(at::Tensor g, at::Tensor u) {
       "Stoke -- swiglu(save_bits=8) takes gate and up of one shape, device "
       "and dtype (bf16, fp16, fp32), got ", g.sizes(), " ", g.scalar_type(),
       " and ", u.sizes(), " ", u.scalar_type());
-  if (at::GradMode::is_enabled()) elem::check_capture({g, u});
+  if (!at::GradMode::is_enabled() || !(g.requires_grad() || u.requires_grad()))
+    return swiglu8_forward(g, u, nullptr);
+  elem::check_capture({g, u});
   return SwiGLU8::apply(g, u);
 }

@@ -8,7 +8,9 @@ import weakref
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
+from stoke import ops
 from stoke.nn import (
     CompressedActivation,
     apply_activation_checkpointing,
@@ -268,6 +270,51 @@ def test_swiglu8_rows_at_any_distance(shape, device):
         want = torch.autograd.grad(yc, (gc, uc), dense)
         assert torch.equal(y, yc)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SIZES + [(0, 8)])
+def test_swiglu8_without_gradient_is_the_same(shape, dtype, device):
+    _skip(device)
+    wide = _act((*shape[:-1], 2 * shape[-1]), dtype, device, 1)
+    for g, u in (wide.chunk(2, -1),
+                 [v.contiguous() for v in wide.chunk(2, -1)]):
+        want = swiglu(g.detach().requires_grad_(True), u, save_bits=8)
+        assert want.requires_grad
+        plain = swiglu(g, u, save_bits=8)
+        with torch.no_grad():
+            scored = swiglu(g.detach().requires_grad_(True), u, save_bits=8)
+        for y in (plain, scored):
+            assert not y.requires_grad
+            assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1 << 20, (65 << 20) + 40])
+def test_gpu_swiglu8_without_gradient_holds_nothing(n):
+    _skip("cuda")
+    g = torch.randn(n, device="cuda", dtype=torch.bfloat16,
+                    generator=torch.Generator("cuda").manual_seed(0))
+    want = swiglu(g.clone().requires_grad_(True), g, save_bits=8).detach()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = swiglu(g, g, save_bits=8)
+    # the output alone, in the allocator's pieces of 2 MB at most
+    assert torch.cuda.max_memory_allocated() - before <= 2 * n + (2 << 20)
+    assert torch.equal(y, want)
+
+
+def test_swiglu8_forward_mode_is_refused_by_the_kernel():
+    if not ops.has_ext():
+        pytest.skip("extension not built")
+    x = torch.ones(40)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, x)
+        for args in ((d, x), (x, d)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops._require_ext().swiglu8(*args)
 
 
 # -------------------------------------------------------------- checkpoints
