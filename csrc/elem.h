@@ -4,10 +4,12 @@
 
 #include <hip/hip_runtime.h>
 
+#include <unordered_set>
+
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/core/StreamGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -49,24 +51,47 @@ inline hipStream_t stream() {
   return at::hip::getCurrentHIPStream().stream();
 }
 
-// A leaf's gradient belongs to the stream on which a graph first reached it,
-// for as long as any graph that does lives.  A backward captured elsewhere
-// would wait there on an event of the capture, which ends the process: such a
-// call is refused in the forward, before anything is recorded.
+// The legacy default stream takes no capture.
+inline bool is_capturing(const c10::Stream& s) {
+  if (s.id() == 0) return false;
+  const c10::StreamGuard guard(s);
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() !=
+         c10::hip::CaptureStatus::None;
+}
+
+// A node of an autograd graph belongs to the stream on which it was recorded,
+// a leaf's to the one on which a graph first reached the leaf, for as long as
+// any graph that does lives.  A backward captured elsewhere would wait there
+// on an event of the capture, which ends the process: a call whose gradients
+// reach such a node is refused in the forward, before anything is recorded.
 inline void check_capture(std::initializer_list<at::Tensor> inputs) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() ==
       c10::hip::CaptureStatus::None)
     return;
+  std::vector<torch::autograd::Node*> next;
+  std::unordered_set<torch::autograd::Node*> seen;
+  std::vector<std::shared_ptr<torch::autograd::Node>> leaves;
+  const auto reach = [&](torch::autograd::Node* node) {
+    if (node && seen.insert(node).second) next.push_back(node);
+  };
   for (const at::Tensor& t : inputs) {
-    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) continue;
+    if (!t.defined() || !t.requires_grad()) continue;
+    if (t.is_leaf()) {
+      leaves.push_back(torch::autograd::impl::try_get_grad_accumulator(t));
+      reach(leaves.back().get());
+    } else {
+      reach(t.grad_fn().get());
+    }
+  }
+  while (!next.empty()) {
+    torch::autograd::Node* node = next.back();
+    next.pop_back();
     const auto at = node->stream();
-    const c10::impl::VirtualGuardImpl guard(t.device().type());
-    TORCH_CHECK(!at || *at == guard.getStream(t.device()),
-                "Stoke -- a graph capture with gradients of a leaf that an "
-                "autograd graph of another stream still holds: drop that "
-                "graph (its outputs and losses) before the capture");
+    TORCH_CHECK(!at || is_capturing(*at),
+                "Stoke -- a graph capture with gradients that reach an "
+                "autograd graph of another stream: drop that graph (its "
+                "outputs and losses) before the capture");
+    for (const auto& edge : node->next_edges()) reach(edge.function.get());
   }
 }
 

@@ -16,6 +16,8 @@ from stoke.nn import (
     apply_activation_checkpointing,
     fused_policy_loss,
     fused_preference_loss,
+    qk_norm_rope,
+    swiglu,
     token_logprobs,
 )
 
@@ -118,6 +120,92 @@ def test_gpu_step_under_autocast_and_in_bf16():
             cos = torch.nn.functional.cosine_similarity(
                 g.float().cpu().flatten(), w.flatten(), dim=0)
             assert float(cos) > 0.9, (name, float(cos))
+
+
+def _operators(w):
+    """Each operator on tensors made of the leaf w [4, 64]."""
+    t = torch.zeros(4, dtype=torch.int64, device=w.device)
+    v = torch.zeros(4, device=w.device)
+    c = torch.ones(4, 8, device=w.device)
+
+    def heads(y):
+        q = y.view(1, 4, 4, 16)
+        return qk_norm_rope(q, q, None, None, c, c)[0]
+
+    return [
+        lambda y: token_logprobs(y, t),
+        lambda y: fused_policy_loss(y, t, v, v),
+        lambda y: fused_preference_loss(y[:, None], t[:, None],
+                                        v[:, None])[0],
+        heads,
+        lambda y: swiglu(y, y, save_bits=8),
+    ]
+
+
+@pytest.mark.gpu
+def test_gpu_capture_over_a_live_graph_behind_other_operators():
+    """The leaf is reached through what was computed in the capture, or the
+    input itself was computed before it."""
+    _skip("cuda")
+    w = torch.randn(4, 64, device="cuda",
+                    generator=torch.Generator("cuda").manual_seed(0))
+    w.requires_grad_(True)
+    alive = w * 2.0  # a graph of the default stream
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        inside = (w * 0.5).view(4, 64)
+        for fn in _operators(w):
+            for y in (inside, alive):
+                with pytest.raises(RuntimeError, match="drop that graph"):
+                    fn(y)
+            with torch.no_grad():
+                out = fn(inside)
+            assert not out.requires_grad
+    del alive, inside, y
+
+
+@pytest.mark.gpu
+def test_gpu_capture_behind_other_operators_and_over_a_fork():
+    _skip("cuda")
+    w = torch.randn(4, 64, device="cuda",
+                    generator=torch.Generator("cuda").manual_seed(0))
+    w.requires_grad_(True)
+
+    def step():
+        outs = [fn((w * 0.5).view(4, 64)) for fn in _operators(w)]
+        return torch.autograd.grad(sum(o.sum() for o in outs), w)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            w.mul_(1.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, step()), i
+    # a stream that the capture has forked belongs to it
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            inside = w * 0.5
+        main.wait_stream(side)
+        outs = [fn(inside) for fn in _operators(w)]
+    assert all(o.requires_grad for o in outs)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = [fn(w.detach() * 0.5) for fn in _operators(w)]
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 @pytest.mark.parametrize("device", DEVICES)
