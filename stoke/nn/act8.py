@@ -110,8 +110,9 @@ class _SwiGLU8Fn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         qg, sg, qu, su = ctx.saved_tensors
-        g = _eager_unpack(qg, sg, torch.float32)
-        u = _eager_unpack(qu, su, torch.float32)
+        # in the inputs' dtype: its range bounds what is read back
+        g = _eager_unpack(qg, sg, dy.dtype).float()
+        u = _eager_unpack(qu, su, dy.dtype).float()
         s, d = torch.sigmoid(g), dy.float()
         return ((d * u * s * (1 + g * (1 - s))).to(dy.dtype),
                 (d * g * s).to(dy.dtype))

@@ -274,6 +274,25 @@ def test_swiglu8_rows_at_any_distance(shape, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [40, 64])
+def test_swiglu8_gradient_at_the_largest_value(n, dtype, device):
+    """8 bits round it to a power of two out of range; it stays the largest."""
+    _skip(device)
+    top = torch.finfo(dtype).max
+    g = torch.zeros(n, dtype=dtype)
+    g[3] = g[-1] = top
+    u = torch.zeros(n, dtype=dtype)
+    g, u = (v.to(device).requires_grad_(True) for v in (g, u))
+    y = swiglu(g, u, save_bits=8)
+    dg, du = torch.autograd.grad(y, (g, u), torch.ones_like(y))
+    want = torch.zeros(n, dtype=dtype)
+    want[3] = want[-1] = top  # silu(top) = top
+    assert torch.equal(du.cpu(), want)
+    assert bool((dg == 0).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", SIZES + [(0, 8)])
 def test_swiglu8_without_gradient_is_the_same(shape, dtype, device):
     _skip(device)
