@@ -147,8 +147,10 @@ def fused_policy_loss(logits: torch.Tensor, actions: torch.Tensor,
 def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
                           ref_logprobs: torch.Tensor, beta: float = 0.1,
                           label_smoothing: float = 0.0,
-                          ignore_index: int = -100):
-    """Paired preference loss; returns ``(loss, rewards)``.
+                          ignore_index: int = -100,
+                          return_rewards: bool = True):
+    """Paired preference loss; returns ``(loss, rewards)``, or the loss alone
+    with ``return_rewards=False``, as ``Stoke(loss=...)`` takes it.
 
     logits: [2P, S, V] and targets [2P, S]: the P chosen sequences, then the
     P rejected ones in the same order.  ref_logprobs: [2P, S], the reference
@@ -163,8 +165,9 @@ def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
     """
     ext = _native(logits)
     if ext is not None:
-        return tuple(ext.preference_loss(logits, targets, ref_logprobs, beta,
-                                         label_smoothing, ignore_index))
+        loss, rewards = ext.preference_loss(
+            logits, targets, ref_logprobs, beta, label_smoothing, ignore_index)
+        return (loss, rewards) if return_rewards else loss
     _check(logits, targets, "fused_preference_loss")
     if logits.dim() != 3 or logits.shape[0] % 2 or logits.shape[0] == 0:
         raise ValueError(
@@ -187,4 +190,5 @@ def fused_preference_loss(logits: torch.Tensor, targets: torch.Tensor,
     if label_smoothing != 0:  # a margin of +inf: not 0 * inf
         loss = loss - label_smoothing * ls(-h)
     dt = _result_dtype(logits)
-    return loss.mean().to(dt), rewards.detach().to(dt)
+    loss = loss.mean().to(dt)
+    return (loss, rewards.detach().to(dt)) if return_rewards else loss

@@ -7,11 +7,13 @@ import os
 import subprocess
 import sys
 from contextlib import nullcontext
+from functools import partial
 
 import pytest
 import torch
 
 from benchmarks.models import LlamaBlock, llama_tiny
+from stoke import Stoke, StokeOptimizer
 from stoke.nn import (
     apply_activation_checkpointing,
     fused_policy_loss,
@@ -120,6 +122,48 @@ def test_gpu_step_under_autocast_and_in_bf16():
             cos = torch.nn.functional.cosine_similarity(
                 g.float().cpu().flatten(), w.flatten(), dim=0)
             assert float(cos) > 0.9, (name, float(cos))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("accum", [1, 2])
+@pytest.mark.parametrize("kind", ["policy", "preference"])
+def test_losses_under_the_facade(kind, accum, device):
+    _skip(device)
+    x, y = _batch(device)
+    adv = torch.tensor([[1.0], [-0.5], [0.3], [-1.0]], device=device)
+    m = _model(8, device, torch.float32)
+    with torch.no_grad():
+        old = token_logprobs(m(x), y)
+    if kind == "policy":
+        loss = partial(fused_policy_loss, kl_coef=0.1)
+        args = (y, old, adv, old - 0.05)
+    else:
+        loss = partial(fused_preference_loss, beta=0.2, return_rewards=False)
+        args = (y, old - 0.05)
+    params = dict(m.named_parameters())
+    want = {n: p.detach().clone() for n, p in params.items()}
+    grads = torch.autograd.grad(loss(m(x), *args), list(params.values()))
+    s = Stoke(
+        model=_model(8, device, torch.float32),
+        optimizer=StokeOptimizer(optimizer=torch.optim.SGD,
+                                 optimizer_kwargs={"lr": 0.5}),
+        loss=loss, batch_size_per_device=4, grad_accum_steps=accum,
+        gpu=device == "cuda", verbose=False)
+    s.model_access.train()
+    for _ in range(accum):  # the same batch: the mean is its gradient
+        value = s.loss(s.model(x), *args)
+        assert value.dim() == 0
+        s.backward(value)
+        s.step()
+    got = s.model_access.state_dict()
+    for (n, p), g in zip(params.items(), grads):
+        # halves of equal gradients add up to them, the step rounds once more;
+        # the library may add a gradient's parts up in another order
+        off = (got[n] - (want[n] - 0.5 * g)).abs()
+        size = want[n].abs() + g.abs()
+        assert bool((off <= 4 * 2.0 ** -24 * size + 1e-6 * g.abs().max()
+                     ).all()), n
+        assert bool((got[n] != want[n]).any()), n
 
 
 def _operators(w):
