@@ -63,7 +63,6 @@ class SyntheticDocs(torch.utils.data.Dataset):
 def pad_collate(batch):
     # inputs pad with 0; TARGETS pad with -100 so padded positions are
     # ignored by the loss instead of trained as real next tokens
-    # 
     L = max(t.numel() for t in batch)
     x = torch.zeros(len(batch), L, dtype=torch.long)
     y = torch.full((len(batch), L), -100, dtype=torch.long)
@@ -79,7 +78,21 @@ def lm_loss(logits, target):
     return fused_cross_entropy(logits, target, ignore_index=-100)
 
 
-def main():
+def build_model(args):
+    nh = max(4, args.dim // 128)
+    # inside a checkpointed block SwiGLU's inputs live for the block's own
+    # backward alone: 8 bits would round a second time for no memory
+    swiglu_bits = 16 if args.act_ckpt else args.act_bits
+    model = Llama(vocab=args.vocab, d=args.dim, nlayer=args.layers, nh=nh,
+                  nkv=max(2, nh // 2), ffn=2 * args.dim, max_seq=512,
+                  qk_norm=args.qk_norm, act_bits=swiglu_bits)
+    if args.act_ckpt:
+        apply_activation_checkpointing(model, min_params=10_000,
+                                       save_bits=args.act_bits)
+    return model
+
+
+def parse_args(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--cpu", action="store_true")
     ap.add_argument("--fsdp", action="store_true")
@@ -92,20 +105,18 @@ def main():
     ap.add_argument("--act-ckpt", action="store_true")
     ap.add_argument("--act-bits", type=int, default=16, choices=(16, 8),
                     help="bits of the activations that wait for the "
-                         "backward: checkpoints and SwiGLU inputs")
+                         "backward: checkpoints, or without them the inputs "
+                         "of SwiGLU")
     ap.add_argument("--qk-norm", action="store_true",
                     help="normalise query and key heads before the rotation")
-    args = ap.parse_args()
+    return ap.parse_args(argv)
 
+
+def main():
+    args = parse_args()
     world = int(os.environ.get("WORLD_SIZE", "1"))
     distributed = world > 1
-    nh = max(4, args.dim // 128)
-    model = Llama(vocab=args.vocab, d=args.dim, nlayer=args.layers, nh=nh,
-                  nkv=max(2, nh // 2), ffn=2 * args.dim, max_seq=512,
-                  qk_norm=args.qk_norm, act_bits=args.act_bits)
-    if args.act_ckpt:
-        apply_activation_checkpointing(model, min_params=10_000,
-                                       save_bits=args.act_bits)
+    model = build_model(args)
 
     s = Stoke(
         model=model,

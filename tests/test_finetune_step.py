@@ -3,6 +3,7 @@
 and preference losses over a decoder with normalised heads, 8-bit SwiGLU
 inputs and 8-bit checkpoints."""
 
+import importlib.util
 import os
 import subprocess
 import sys
@@ -265,3 +266,20 @@ def test_example_runs(device):
                        text=True, timeout=110)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
     assert "done: 2 steps" in r.stdout
+
+
+@pytest.mark.parametrize("flags,swiglu_bits", [
+    ("--act-bits 8", 8), ("--act-bits 8 --act-ckpt", 16), ("--act-ckpt", 16),
+    ("", 16)])
+def test_example_holds_an_activation_once(flags, swiglu_bits):
+    """SwiGLU inputs inside a recomputed block stay as they are."""
+    spec = importlib.util.spec_from_file_location(
+        "llm_train", os.path.join(REPO, "examples", "llm", "train.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    m = ex.build_model(ex.parse_args(
+        ["--layers", "2", "--dim", "256", *flags.split()]))
+    assert [b.act_bits for b in m.blocks] == [swiglu_bits] * 2
+    held = [getattr(b, "_stoke_act_ckpt_bits", None) for b in m.blocks]
+    bits = 8 if "8" in flags else 16
+    assert held == ([bits] * 2 if "--act-ckpt" in flags else [None] * 2)
