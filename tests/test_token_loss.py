@@ -306,6 +306,87 @@ def test_gpu_logprobs_have_no_bias(dtype):
     assert float(off.std()) < 4e-7
 
 
+def _lp_errors(x, t, per_call):
+    """lp - float64 of single tokens, past the rounding to fp32: a sequence of
+    one token has the reward lp - ref, and next to lp a reference leaves a
+    reward of at most U |lp|, which fp32 holds to 1e-13."""
+    off = []
+    for i in range(0, len(x), per_call):
+        y, at = x[i:i + per_call].double(), t[i:i + per_call, None]
+        want = (y.gather(1, at) - torch.logsumexp(y, -1, True))[:, 0]
+        ref = want.float()
+        _, r = fused_preference_loss(x[i:i + per_call, None], at,
+                                     ref[:, None], beta=1.0)
+        off.append(r.double() + ref.double() - want)
+    return torch.cat(off)
+
+
+def _lp_model(x):
+    """What the roundings of lp come to: the mean square over the rows, and
+    the variance of the mean.
+
+    Relative to a term p are off the argument a of exp2, by half an ulp of it
+    at most, and exp2, by an ulp at most, both taken as even over their range
+    (a third of the square), and 5 levels of fp32 sums of 32 values, U each,
+    over groups that hold 32 / V of the row by their other values.  The
+    largest term is exact, and so is the sum next to it.  In 16 bits the rows
+    share their values, and a value is off the same way in each: it counts in
+    the mean with its share of all rows."""
+    v = x.shape[1]
+    square, mass, worst = 0.0, {}, {}
+    for i in range(0, len(x), 256):
+        y = x[i:i + 256].double()
+        p = torch.softmax(y, -1)
+        top = p.argmax(-1, True)
+        rest = 1 - p.gather(1, top)
+        # a is relative to a whole number up to 1 above the maximum
+        a = (y.gather(1, top) - y) * 1.4426950408889634 + 1
+        ulp = 2.0 ** (torch.log2(a).floor() - 23)
+        var = (0.6931 * ulp / 2) ** 2 / 3 + (2 * U) ** 2 / 3
+        p = p.scatter(1, top, 0.0)
+        square += float((p * p * (var + 5 * U * U / 3)).sum())
+        square += float((rest ** 2).sum()) * 32 / v * 5 * U * U / 3
+        if x.dtype == torch.float32:
+            continue
+        vals, inv = x[i:i + 256].float().unique(return_inverse=True)
+        inv = inv.flatten()
+        m = torch.zeros_like(vals, dtype=torch.float64)
+        m = m.index_add(0, inv, p.flatten())
+        w = torch.zeros_like(m).scatter_reduce(0, inv, var.flatten(), "amax")
+        for u, b, c in zip(vals.tolist(), m.tolist(), w.tolist()):
+            mass[u] = mass.get(u, 0.0) + b
+            worst[u] = max(worst.get(u, 0.0), c)
+    n = len(x)
+    shared = sum(mass[u] ** 2 * worst[u] for u in mass) / n / n
+    return square / n, square / n / n + shared
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("peaked", [False, True])
+@pytest.mark.parametrize("per_call", [1024, 32])  # rows whole and in 32 pieces
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gpu_rewards_have_no_bias_that_sequences_add_up(dtype, per_call,
+                                                        peaked):
+    _skip("cuda")
+    rows, v = 1024, 128256
+    gen = torch.Generator("cuda").manual_seed(0)
+    x = torch.randn(rows, v, device="cuda", generator=gen)
+    t = torch.randint(0, v, (rows,), device="cuda", generator=gen)
+    if peaked:  # one token has half of the weight to almost all of it
+        at = torch.randint(0, v, (rows, 1), device="cuda", generator=gen)
+        lse = torch.logsumexp(x, -1, True)
+        x.scatter_(1, at, lse + 4 * torch.rand(rows, 1, device="cuda",
+                                               generator=gen))
+    else:
+        x *= 2.5
+    x = x.to(dtype)
+    off = _lp_errors(x, t, per_call)
+    square, mean = _lp_model(x)
+    assert float(off.std()) <= square ** 0.5
+    # the bias of exp2, 3.2e-9, is given back to a third of it, 4 deviations
+    assert abs(float(off.mean())) <= 1e-9 + 4 * mean ** 0.5
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_rows_without_a_distribution_are_nan(device):
     _skip(device)
