@@ -76,7 +76,7 @@ __device__ __forceinline__ float exp_of(float d) {
 // than 1e-9 on average, in every type.
 struct Part {
   double sum;
-  float max, k, moment, unused;
+  float max, k, moment;
 };
 
 template <bool BF16>
@@ -92,7 +92,7 @@ constexpr float kHuge = BF16 ? 8192.f : 536870912.f;
 constexpr float kLeast = -1e9f;  // first k
 
 __device__ __forceinline__ Part nothing() {
-  return Part{0., -__builtin_huge_valf(), kLeast, 0.f, 0.f};
+  return Part{0., -__builtin_huge_valf(), kLeast, 0.f};
 }
 
 template <bool BF16>
@@ -127,7 +127,7 @@ __device__ __forceinline__ void join(Part& p, const Part& q) {
 
 __device__ __forceinline__ Part from_lane(const Part& p, int off) {
   return Part{__shfl_xor(p.sum, off), __shfl_xor(p.max, off),
-              __shfl_xor(p.k, off), __shfl_xor(p.moment, off), 0.f};
+              __shfl_xor(p.k, off), __shfl_xor(p.moment, off)};
 }
 
 // Elements of `row` up to the first 16-byte boundary.
