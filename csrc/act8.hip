@@ -1,4 +1,4 @@
-// Activations held in 8 bits (MXINT8: 32 values share a power of two).
+// Activations held in 8 bits: 32 values share a power of two.
 //
 // A block of 32 consecutive values of the flattened tensor keeps one byte
 // E and 32 signed bytes q with  value = q * 2^(E - 127),  |q| <= 127.

@@ -762,8 +762,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused AdamW, bf16 params + fp32 master (HIP)");
   m.def("amp_update_scale_", &amp_update_scale_,
         "dynamic loss scale update (HIP)");
-  m.def("act8_pack", &act8_pack, "activation to 8 bits (MXINT8)");
-  m.def("act8_unpack", &act8_unpack, "activation back from 8 bits (MXINT8)");
+  m.def("act8_pack", &act8_pack, "activation to 8 bits");
+  m.def("act8_unpack", &act8_unpack, "activation back from 8 bits");
   m.def("swiglu8", &swiglu8,
         "silu(g)*u, keeping g and u in 8 bits for the backward");
   m.def("token_logprobs", &token_logprobs,

@@ -1,11 +1,14 @@
 # -*- coding: utf-8 -*-
 """Activations held in 8 bits between the forward and the backward pass.
 
-The format is MXINT8: 32 consecutive values of the flattened tensor share a
-power of two (one byte ``E``) and keep a signed byte each, so that
-``value = q * 2**(E - 127)``.  It costs 1 1/32 bytes a value; a value is off
-by at most 1/127 of the largest of its 32.  A block with an infinity or NaN
-(``E = 255``) reads back as NaN, so overflows still reach the gradients.
+32 consecutive values of the flattened tensor share a power of two (one byte
+``E``) and keep a signed byte each, so that ``value = q * 2**(E - 127)``.  It
+costs 1 1/32 bytes a value; a value is off by at most 1/127 of the largest of
+its 32, or by 2^-127 where that one is below 2^-120.  A block with an infinity
+or NaN (``E = 255``) reads back as NaN, so overflows still reach the gradients.
+The published microscaling format of 8-bit integers looks alike, but its bytes
+stand for ``q * 2**(E - 133)`` and its exponent is chosen by another rule: one
+does not read the other.
 
 ``compress_activation`` / ``restore_activation`` are the format itself,
 ``apply_activation_checkpointing(..., save_bits=8)`` keeps a block's inputs

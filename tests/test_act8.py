@@ -114,6 +114,21 @@ def test_format_at_the_ends_of_the_range(dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e-35, 1e-36, 1e-37, 1e-38, 1e-39])
+def test_bound_of_tiny_blocks(size, dtype, device):
+    _skip(device)
+    g = torch.Generator().manual_seed(0)
+    x = (size * torch.randn(40, 32, generator=g).double()).to(dtype)
+    back = restore_activation(compress_activation(x.to(device))).cpu()
+    off = (back.double() - x.double()).abs()
+    top = x.double().abs().amax(-1, keepdim=True)
+    bound = torch.where(top < 2.0 ** -120, torch.full_like(top, 2.0 ** -127),
+                        top / 127)
+    assert bool((off <= bound).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
 def test_non_finite_blocks_read_back_as_nan(bad, dtype, device):
