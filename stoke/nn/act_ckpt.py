@@ -101,8 +101,13 @@ def _holds(t) -> bool:
 
 
 def _first_parameter(forward) -> Optional[str]:
-    """Name of the argument that holds a block's input."""
-    for p in inspect.signature(forward).parameters.values():
+    """Name of the argument that holds a block's input, for calls that give it
+    by name."""
+    try:
+        params = inspect.signature(forward).parameters.values()
+    except (TypeError, ValueError):  # compiled code may have none
+        return None
+    for p in params:
         return p.name if p.kind is p.POSITIONAL_OR_KEYWORD else None
     return None
 

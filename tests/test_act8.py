@@ -561,6 +561,22 @@ def test_checkpoint8_leaves_biases_and_masks_exact(by_name, mask, device):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+def test_checkpoint8_of_a_forward_without_a_signature(bits):
+    class Tanh(torch.nn.Module):
+        forward = staticmethod(torch.tanh)
+
+    net = torch.nn.Sequential(Tanh())
+    apply_activation_checkpointing(net, predicate=lambda n, m: True,
+                                   save_bits=bits)
+    leaf = torch.linspace(-1, 1, 33).mul(64).round().div(64)
+    leaf.requires_grad_(True)
+    net(leaf * 1.0).sum().backward()
+    want = 1 - leaf.detach().double().tanh().square()
+    # tanh to 2 ulp, its square twice that, and three more roundings
+    assert bool(((leaf.grad.double() - want).abs() <= 8 * 2.0 ** -24).all())
+
+
 def test_checkpoint8_input_that_comes_twice():
     x = (torch.randint(-127, 128, (8, 32),
                        generator=torch.Generator().manual_seed(1)) / 64)
