@@ -469,7 +469,7 @@ at::Tensor act8_unpack(at::Tensor values, at::Tensor scales,
 
 // The entry point: checks its arguments, and has gradients for both.
 at::Tensor swiglu8(at::Tensor g, at::Tensor u) {
-  elem::refuse_tangents("swiglu(save_bits=8)", {g, u});
+  elem::refuse_tangents("swiglu(save_bits=8)", g, u);
   TORCH_CHECK_VALUE(
       g.is_cuda() && g.sizes() == u.sizes() && g.device() == u.device() &&
           g.scalar_type() == u.scalar_type() &&

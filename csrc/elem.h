@@ -98,12 +98,16 @@ inline void check_capture(std::initializer_list<at::Tensor> inputs) {
 // A forward-mode tangent would be dropped where a kernel runs without an
 // autograd node: an input that carries one is refused.  (The node itself
 // refuses it too.)
-inline void refuse_tangents(const char* what,
-                            std::initializer_list<at::Tensor> inputs) {
-  for (const at::Tensor& t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(
-        !t.defined() || !t._fw_grad(/*level=*/0).defined(), "Stoke -- ", what,
-        " has no forward-mode derivative on the GPU");
+inline bool has_tangent(const at::Tensor& t) {
+  return t.defined() && t._fw_grad(/*level=*/0).defined();
+}
+inline bool has_tangent(const std::optional<at::Tensor>& t) {
+  return t && has_tangent(*t);
+}
+template <typename... Inputs>
+void refuse_tangents(const char* what, const Inputs&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "Stoke -- ", what,
+                              " has no forward-mode derivative on the GPU");
 }
 
 // Gradients of a kernel without a derivative of its own: a second backward

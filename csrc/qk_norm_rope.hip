@@ -943,9 +943,7 @@ std::vector<at::Tensor> qk_norm_rope(
     std::optional<at::Tensor> pos,
     std::optional<std::vector<int64_t>> sections, double eps,
     bool interleaved) {
-  elem::refuse_tangents("qk_norm_rope",
-                        {q, k, wq.value_or(at::Tensor()),
-                         wk.value_or(at::Tensor()), cosines, sines});
+  elem::refuse_tangents("qk_norm_rope", q, k, wq, wk, cosines, sines);
   Tensors t;
   if (wq) t.wq = wq->contiguous();
   if (wk) t.wk = wk->contiguous();

@@ -971,7 +971,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
 // The entry points check their arguments and have gradients for the logits.
 at::Tensor token_logprobs(at::Tensor logits, at::Tensor target,
                           int64_t ignore) {
-  elem::refuse_tangents("token_logprobs", {logits});
+  elem::refuse_tangents("token_logprobs", logits);
   check(logits, target, "token_logprobs");
   const auto x = rows_of(logits), t = target.contiguous();
   if (!wants_grad(logits)) return logprobs_forward(x, t, ignore, at::Tensor());
@@ -982,8 +982,7 @@ at::Tensor policy_loss(at::Tensor logits, at::Tensor target,
                        at::Tensor old_lp, at::Tensor adv,
                        std::optional<at::Tensor> ref_lp, double clip_low,
                        double clip_high, double kl, int64_t ignore) {
-  elem::refuse_tangents("fused_policy_loss",
-                        {logits, old_lp, adv, ref_lp.value_or(at::Tensor())});
+  elem::refuse_tangents("fused_policy_loss", logits, old_lp, adv, ref_lp);
   check(logits, target, "fused_policy_loss");
   TORCH_CHECK_VALUE(
       clip_low >= 0 && clip_low <= 1 && clip_high >= 0 && kl >= 0,
@@ -1008,7 +1007,7 @@ at::Tensor policy_loss(at::Tensor logits, at::Tensor target,
 std::vector<at::Tensor> preference_loss(at::Tensor logits, at::Tensor target,
                                         at::Tensor ref_lp, double beta,
                                         double eps, int64_t ignore) {
-  elem::refuse_tangents("fused_preference_loss", {logits, ref_lp});
+  elem::refuse_tangents("fused_preference_loss", logits, ref_lp);
   check(logits, target, "fused_preference_loss");
   TORCH_CHECK_VALUE(
       logits.dim() == 3 && logits.size(0) > 0 && logits.size(0) % 2 == 0,
