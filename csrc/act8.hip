@@ -146,11 +146,12 @@ __device__ __forceinline__ void swiglu_grad(float d, float a, float b,
 // backward, written).  What the forward writes is read by the next product:
 // it goes through them.
 //
-// All are bound by memory: 134M bf16 values pack in 62 us and unpack in 60 us
-// (407 MB each, 6.6 and 6.8 TB/s; 69 and 68 us through the caches); SwiGLU
-// at 8192 x 14336 takes 150 us forward (947 MB, 6.3 TB/s; 160 us) and 152 us
-// backward (6.2 TB/s; 163 us).  One value a thread took 389 and 659 us for
-// both directions.
+// All are bound by memory.  Two runs of 134M bf16 values packed in 68 and 74 us
+// and unpacked in 59 and 64 us (407 MB each, 5.5 to 6.9 TB/s); SwiGLU at 8192 x
+// 14336 took 156 and 168 us forward (947 MB, 5.6 to 6.1 TB/s; 109 us and 705 MB
+// without a backward to come) and 154 and 166 us backward.  Through the caches
+// they took 7 to 13 % longer.  One value a thread took 389 and 659 us for both
+// directions, against 133 and 309 us.
 template <typename T, bool NT>
 __global__ __launch_bounds__(kThreads) void pack_kernel(
     const T* __restrict__ x, signed char* __restrict__ q,
@@ -425,7 +426,7 @@ std::vector<at::Tensor> act8_pack(at::Tensor act) {
   auto scale = at::empty({(n + 31) / 32}, x.options().dtype(at::kByte));
   STOKE_ELEM_SWITCH(x.scalar_type(), "act8_pack", {
     const long first = first_of(n);
-    // past the caches a thread takes two runs: 134M values 63 against 67 us
+    // past the caches a thread takes two runs: 134M values in 6 % less time
     if (n > 0)
       with_caching(n * (long)sizeof(T), [&](auto nt) {
         hipLaunchKernelGGL((pack_kernel<T, nt>),
