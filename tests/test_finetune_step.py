@@ -211,6 +211,32 @@ def test_gpu_capture_over_a_live_graph_behind_other_operators():
 
 
 @pytest.mark.gpu
+def test_gpu_capture_over_a_live_graph_of_a_side_stream():
+    """A warm-up whose result was kept: its stream takes no part in the
+    capture."""
+    _skip("cuda")
+    w = torch.randn(4, 64, device="cuda",
+                    generator=torch.Generator("cuda").manual_seed(0))
+    w.requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = w * 2.0
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = w * 0.5
+        for fn in _operators(w):
+            for y in (inside, alive):
+                with pytest.raises(RuntimeError, match="drop that graph"):
+                    fn(y)
+        out = inside.detach() + 1
+    graph.replay()
+    assert torch.equal(out, w.detach() * 0.5 + 1)
+
+
+@pytest.mark.gpu
 def test_gpu_capture_behind_other_operators_and_over_a_fork():
     _skip("cuda")
     w = torch.randn(4, 64, device="cuda",
