@@ -246,8 +246,8 @@ __device__ __forceinline__ RowLp finish(const Part& p, float xt) {
 // piece a row) a row's lp is written here.
 //
 // Bound by memory: 8192 rows of 128256 bf16, 65 % of them read, take 237 us
-// (1.37 GB, 5.8 TB/s), all of them 376 us.  A thread takes 32 values between two looks at its
-// maximum; the loads stay in the caches for the backward.
+// (1.37 GB, 5.8 TB/s), all of them 376 us.  A thread takes 32 values between two
+// looks at its maximum; the loads stay in the caches for the backward.
 template <typename T, int THREADS, bool FINISH>
 __global__ __launch_bounds__(THREADS) void row_stats_kernel(
     const T* __restrict__ logits, const long* __restrict__ target,

@@ -68,8 +68,8 @@ if __name__ == "__main__":
                 depends=["csrc/elem.h"],
                 extra_compile_args={
                     "cxx": ["-O3"],
-                    # scalar fp32 only: some packed fp32 forms the compiler makes
-                    # by itself are not reliable on this target
+                    # scalar fp32 only: some packed fp32 forms that the compiler
+                    # makes by itself are not reliable on this target
                     "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
                              "-Xclang", "-packed-fp32-ops"],
                 },
